@@ -1,5 +1,5 @@
 """Phase timeline of the fused inverted-residual BACKWARD kernel from in-kernel clock stamps (diagnostic build tools/micro/lib_sirdbg.so:
-hipcc --offload-arch=gfx950 -O3 -std=c++17 -fPIC -shared -DSIR_STAMPS -I diffusion-model_amd/csrc -I include diffusion-model_amd/csrc/*.hip).  python tools/micro/dbg_sir_bwd.py"""
+hipcc --offload-arch=gfx950 -Xclang -target-feature -Xclang -packed-fp32-ops -O3 -std=c++17 -fPIC -shared -DSIR_STAMPS -I diffusion-model_amd/csrc -I include diffusion-model_amd/csrc/*.hip).  python tools/micro/dbg_sir_bwd.py"""
 import sys, os, ctypes
 ROOT = os.path.dirname(os.path.dirname(os.path.dirname(os.path.abspath(__file__))))
 sys.path.insert(0, ROOT); sys.path.insert(0, os.path.join(ROOT, "tests"))

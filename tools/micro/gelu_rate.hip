@@ -1,6 +1,6 @@
 // VALU cost of the activation arithmetic, no memory traffic: every thread evaluates ITER x 8 values held in registers.
 // Prints nanoseconds per launch and the implied SIMD cycles per wave-wide evaluation (at the clock given as argv[1], GHz).
-//   hipcc --offload-arch=gfx950 -O3 -std=c++17 -I diffusion-model_amd/csrc -I include tools/micro/gelu_rate.hip -o tools/micro/gelu_rate
+//   hipcc --offload-arch=gfx950 -Xclang -target-feature -Xclang -packed-fp32-ops -O3 -std=c++17 -I diffusion-model_amd/csrc -I include tools/micro/gelu_rate.hip -o tools/micro/gelu_rate
 #include <hip/hip_runtime.h>
 #include <cstdio>
 #include <cstdlib>

@@ -1,6 +1,6 @@
 // Measured peaks of the device this runs on, for pricing the roofline against what the machine delivers as well as
 // against the vendor figures: HBM read, HBM copy (read + write) and dense bf16 MFMA (v_mfma_f32_32x32x16_bf16).
-// Build: hipcc --offload-arch=gfx950 -O3 -o tools/peaks/peaks tools/peaks/peaks.hip      Run: tools/peaks/peaks
+// Build: hipcc --offload-arch=gfx950 -Xclang -target-feature -Xclang -packed-fp32-ops -O3 -o tools/peaks/peaks tools/peaks/peaks.hip      Run: tools/peaks/peaks
 #include <hip/hip_runtime.h>
 #include <cstdio>
 #include <cstdlib>
