@@ -89,10 +89,17 @@ extern "C" int ddpm_remap(const ddpm_remap_entry* entries, const int32_t* chunks
 // Adam with bias correction (torch.optim.Adam semantics, weight_decay = L2 added to the gradient), plus an optional
 // exponential moving average ema = lerp(ema, p, 1 - ema_decay) of the updated parameters
 // (torch.optim.swa_utils.AveragedModel with get_ema_multi_avg_fn: its first update copies the parameters).  step: device int64, incremented here by the first thread.
+// norm: NULL, or the gradients' global norm: they are then clipped on the way, i.e. grad_scale times min(1, max_norm / (norm + 1e-6)),
+// the norm taken of the scaled gradients; a pass that writes clipped gradients back does not happen.
 __global__ __launch_bounds__(256) void adam_kernel(float* __restrict__ p, const float* __restrict__ g, float* __restrict__ m,
                                                     float* __restrict__ v, float* __restrict__ ema, long long n,
                                                     const float* __restrict__ lr_ptr, float lr_host, float b1, float b2, float eps,
-                                                    float wd, float ema_decay, float grad_scale, long long* __restrict__ step) {
+                                                    float wd, float ema_decay, float grad_scale, long long* __restrict__ step, const float* __restrict__ norm,
+                                                    float max_norm) {
+    if (norm) {
+        const float ratio = max_norm / (*norm * fabsf(grad_scale) + 1e-6f);
+        grad_scale *= ratio > 1.f ? 1.f : ratio;           // (a NaN stays one)
+    }
     const long long st = *step + 1;
     const float lr = lr_ptr ? *lr_ptr : lr_host;
     const float c1 = 1.0f - powf(b1, (float)st), c2 = 1.0f - powf(b2, (float)st);
@@ -119,21 +126,33 @@ __global__ __launch_bounds__(256) void adam_kernel(float* __restrict__ p, const 
 
 __global__ void bump_step_kernel(long long* step) { *step += 1; }
 
-extern "C" int ddpm_adam_step_range(float* p, const float* g, float* m, float* v, float* ema, int64_t n, const float* lr_dev, float lr,
-                                    float beta1, float beta2, float eps, float weight_decay, float ema_decay, float grad_scale,
-                                    int64_t* step, int bump, ddpm_stream_t stream_) {
-    hipStream_t stream = (hipStream_t)stream_;
+static int adam_launch(float* p, const float* g, float* m, float* v, float* ema, int64_t n, const float* lr_dev, float lr, float beta1, float beta2,
+                       float eps, float weight_decay, float ema_decay, float grad_scale, int64_t* step, int bump, const float* norm, float max_norm,
+                       hipStream_t stream) {
     DDPM_REQUIRE(p && g && m && v && step && n > 0 && n % 4 == 0, "adam: bad arguments (n must be a multiple of 4)");
     long long gx = (n / 4 + 255) / 256;
     if (gx > 2048) gx = 2048;
     hipLaunchKernelGGL(adam_kernel, dim3((unsigned)gx), dim3(256), 0, stream, p, g, m, v, ema, (long long)n, lr_dev, lr, beta1, beta2, eps,
-                       weight_decay, ema_decay, grad_scale, (long long*)step);
+                       weight_decay, ema_decay, grad_scale, (long long*)step, norm, max_norm);
     if (bump) hipLaunchKernelGGL(bump_step_kernel, dim3(1), dim3(1), 0, stream, (long long*)step);
     return ddpm_check_launch("adam");
+}
+
+extern "C" int ddpm_adam_step_range(float* p, const float* g, float* m, float* v, float* ema, int64_t n, const float* lr_dev, float lr,
+                                    float beta1, float beta2, float eps, float weight_decay, float ema_decay, float grad_scale,
+                                    int64_t* step, int bump, ddpm_stream_t stream) {
+    return adam_launch(p, g, m, v, ema, n, lr_dev, lr, beta1, beta2, eps, weight_decay, ema_decay, grad_scale, step, bump, nullptr, 0.f, (hipStream_t)stream);
 }
 
 extern "C" int ddpm_adam_step(float* p, const float* g, float* m, float* v, float* ema, int64_t n, const float* lr_dev, float lr,
                               float beta1, float beta2, float eps, float weight_decay, float ema_decay, float grad_scale,
                               int64_t* step, ddpm_stream_t stream) {
     return ddpm_adam_step_range(p, g, m, v, ema, n, lr_dev, lr, beta1, beta2, eps, weight_decay, ema_decay, grad_scale, step, 1, stream);
+}
+
+extern "C" int ddpm_adam_step_clipped(float* p, const float* g, float* m, float* v, float* ema, int64_t n, const float* lr_dev, float lr,
+                                      float beta1, float beta2, float eps, float weight_decay, float ema_decay, float grad_scale,
+                                      int64_t* step, const float* norm, float max_norm, ddpm_stream_t stream) {
+    DDPM_REQUIRE(norm && max_norm >= 0.f, "adam: the clipped step needs the gradients' norm and a limit that is not negative");
+    return adam_launch(p, g, m, v, ema, n, lr_dev, lr, beta1, beta2, eps, weight_decay, ema_decay, grad_scale, step, 1, norm, max_norm, (hipStream_t)stream);
 }

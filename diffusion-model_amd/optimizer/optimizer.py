@@ -7,10 +7,11 @@ from __future__ import annotations
 
 from typing import Iterable, List, Optional
 
+import numpy as np
 import torch
 from torch import Tensor
 
-from ..runtime import hip
+from ..runtime import hip, ops
 from ..runtime.params import bump_weight_epoch, flat_grad_view
 
 
@@ -25,14 +26,23 @@ class FusedAdam(torch.optim.Optimizer):
     captured step() cannot look at host values when it is replayed: call sync_lr() (or set_lr) after scheduler.step();
     the graph drivers in runtime/graphs.py do so before every replay.
 
+    max_grad_norm: clip the gradients' global 2-norm (times grad_scale, if step() is given one) to this value, as
+    clip_grad_norm_(parameters, max_grad_norm) before the step would; the update reads the norm and scales the gradients on the way,
+    so .grad keeps its values and no pass writes clipped ones.  `grad_norm` holds the last step's norm before clipping (a 0-dim
+    tensor on the device).  The norm needs every gradient: step_ranges() refuses.
+
     One hyper-parameter set for all parameters: several param groups are accepted only when their lr, betas, eps and
     weight_decay agree."""
 
     def __init__(self, params: Iterable[Tensor], lr: float = 1e-3, betas=(0.9, 0.999), eps: float = 1e-8, weight_decay: float = 0.0,
-                 ema_decay: Optional[float] = None, **_ignored):
+                 ema_decay: Optional[float] = None, max_grad_norm: Optional[float] = None, **_ignored):
+        if max_grad_norm is not None and not max_grad_norm >= 0:
+            raise ValueError(f"FusedAdam: max_grad_norm must not be negative, got {max_grad_norm}")
         defaults = dict(lr=lr, betas=betas, eps=eps, weight_decay=weight_decay)
         super().__init__(params, defaults)
         self.ema_decay = ema_decay
+        self.max_grad_norm = max_grad_norm
+        self.grad_norm: Optional[Tensor] = None
         self._flat = None
         self._lr_host = None
         self._check_groups()
@@ -77,6 +87,11 @@ class FusedAdam(torch.optim.Optimizer):
         self._step = torch.zeros(1, device=dev, dtype=torch.long)
         self._lr_host = float(self.param_groups[0]["lr"])
         self._lr = torch.full((1,), self._lr_host, device=dev, dtype=torch.float32)
+        # the gradients' spans of the flat layout (what lies between them need not be zero in a buffer of somebody else's)
+        self._span_off, self._span_n, self._span_kind = ops._merge_spans(
+            np.array(offs, dtype=np.uint64) * np.uint64(4), np.array([p.numel() for p in ps], dtype=np.int64),
+            np.full(len(ps), hip.DTYPE[torch.float32], dtype=np.uint8))
+        self.grad_norm = torch.zeros((), device=dev, dtype=torch.float32) if self.max_grad_norm is not None else None
 
     def set_lr(self, lr: float) -> None:
         for g in self.param_groups:
@@ -127,9 +142,16 @@ class FusedAdam(torch.optim.Optimizer):
         g = self._flat_grad(ps)
         grp = self.param_groups[0]
         b1, b2 = grp["betas"]
-        hip.call("ddpm_adam_step", hip.ptr(self._flat), hip.ptr(g), hip.ptr(self._m), hip.ptr(self._v), hip.ptr(self._ema), self._total,
-                 hip.ptr(self._lr), float(grp["lr"]), float(b1), float(b2), float(grp["eps"]), float(grp["weight_decay"]),
-                 float(self.ema_decay if self.ema_decay is not None else 0.0), float(grad_scale), hip.ptr(self._step), hip.stream())
+        args = (hip.ptr(self._flat), hip.ptr(g), hip.ptr(self._m), hip.ptr(self._v), hip.ptr(self._ema), self._total,
+                hip.ptr(self._lr), float(grp["lr"]), float(b1), float(b2), float(grp["eps"]), float(grp["weight_decay"]),
+                float(self.ema_decay if self.ema_decay is not None else 0.0), float(grad_scale), hip.ptr(self._step))
+        if self.max_grad_norm is None:
+            hip.call("ddpm_adam_step", *args, hip.stream())
+        else:
+            if self.grad_norm is None:                    # (max_grad_norm set after the first step)
+                self.grad_norm = torch.zeros((), device=g.device, dtype=torch.float32)
+            ops.launch_grad_norm(self._span_off + np.uint64(g.data_ptr()), self._span_n, self._span_kind, hip.NORM_L2, None, self.grad_norm)
+            hip.call("ddpm_adam_step_clipped", *args, hip.ptr(self.grad_norm), float(self.max_grad_norm), hip.stream())
         bump_weight_epoch()               # the update happened outside torch's view: invalidate cached weight copies
         return loss
 
@@ -139,6 +161,8 @@ class FusedAdam(torch.optim.Optimizer):
         of 4, e.g. GradStore.unpack_phase / unpack_where ranges), for a driver whose gradients become final in parts.  The
         update is element-wise, so the pieces of one step together give exactly step()'s numbers; the pieces must be
         disjoint, cover every parameter once per step, and only the last call says last=True (it advances the step count)."""
+        if self.max_grad_norm is not None:
+            raise RuntimeError("FusedAdam.step_ranges: clipping needs the norm of all gradients, which a step in pieces does not have; use step()")
         if self._flat is None:
             self._flatten()
         ps = self._params()

@@ -203,7 +203,9 @@ class PipelinedTrainStep:
         # the end of the step, which nothing hides: half the Adam launch and half the re-layout leave the step's tail
         # (2.707 -> 2.695 ms at 32x32x1, 4.99 -> 4.96 ms at 64x64x3).  DDPM_EARLY_ADAM=2 also updates the deep encoder stages
         # one phase before the end: measured slower, that phase's leaf work is what the last phase's leaf work waits for.
-        self._early = not self._sep_adam and four and os.environ.get("DDPM_EARLY_ADAM", "1") != "0"
+        # An optimizer that clips by the global gradient norm needs every gradient first: its step stays whole, at the end.
+        self._early = (not self._sep_adam and four and os.environ.get("DDPM_EARLY_ADAM", "1") != "0"
+                       and getattr(optimizer, "max_grad_norm", None) is None)
         self._early_late = self._early and os.environ.get("DDPM_EARLY_ADAM", "1") == "2"
         if self._early:
             # (the gradients of the deep encoder stages go to torch layout one phase before the end either way: that launch is

@@ -5,6 +5,7 @@ raises RuntimeError with the library's message when an entry point reports an er
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes as C
 import os
 
@@ -88,6 +89,15 @@ class SampleNormDesc(C.Structure):
     _fields_ = [("a", _vp), ("b", _vp), ("gamma", _vp), ("beta", _vp), ("y", _vp), ("stats", _vp), ("dy", _vp), ("du", _vp), ("da", _vp),
                 ("part", _vp), ("N", C.c_int32), ("S", C.c_int32), ("C", C.c_int32), ("act", C.c_int32), ("eps", _f),
                 ("act_beta", _vp), ("dbeta_part", _vp)]
+
+
+class LayerNormDesc(C.Structure):
+    _fields_ = [(k, _vp) for k in ("x", "dy", "y", "dx", "w", "b", "stats", "part", "dw", "db")] + [
+        (k, _i64) for k in ("rows", "ldx", "ldy", "lddy", "lddx")] + [("C", C.c_int32), ("dtype", C.c_int32), ("eps", _f)]
+
+
+DTYPE = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
+NORM_L2, NORM_INF = 0, 1
 
 
 class ReduceEntry(C.Structure):
@@ -189,6 +199,12 @@ _PROTOS = {
     "ddpm_attention_backward": ([_vp, _vp], _i),
     "ddpm_sample_norm_forward": ([_vp, _vp], _i),
     "ddpm_sample_norm_backward": ([_vp, _vp], _i),
+    "ddpm_layer_norm_part_rows": ([C.POINTER(LayerNormDesc)], _i),
+    "ddpm_layer_norm_forward": ([C.POINTER(LayerNormDesc), _vp], _i),
+    "ddpm_layer_norm_backward": ([C.POINTER(LayerNormDesc), _vp], _i),
+    "ddpm_grad_norm_work_bytes": ([_i, _vp], _i64),
+    "ddpm_grad_norm": ([_vp, _vp, _vp, _i, _i, _i, _f, _vp, _vp, _vp], _i),
+    "ddpm_adam_step_clipped": ([_vp, _vp, _vp, _vp, _vp, _i64, _vp, _f, _f, _f, _f, _f, _f, _f, _vp, _vp, _f, _vp], _i),
     "ddpm_dropout_masks": ([_vp, _vp, _i, _i64, _f, _vp, _vp], _i),
 }
 
@@ -227,6 +243,14 @@ def ptr(t):
 def stream() -> int:
     """The hipStream_t torch currently enqueues on (so launches are captured by torch.cuda graphs too)."""
     return torch.cuda.current_stream().cuda_stream
+
+
+def on_device_of(t):
+    """Context in which launches go to the tensor's device (the current one needs no switch)."""
+    return _HERE_ALREADY if t.device.index == torch.cuda.current_device() else torch.cuda.device(t.device)
+
+
+_HERE_ALREADY = contextlib.nullcontext()
 
 
 def call(name: str, *args) -> None:

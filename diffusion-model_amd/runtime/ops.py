@@ -540,6 +540,113 @@ def sample_norm_backward(a: Tensor, b: Optional[Tensor], dy: Tensor, act: int, g
     return du, (da if act else du)
 
 
+def _ln_desc(x: Tensor, w: Optional[Tensor], b: Optional[Tensor], stats: Optional[Tensor], eps: float, **more) -> hip.LayerNormDesc:
+    rows, c = x.shape
+    if x.dtype not in hip.DTYPE:
+        raise ValueError(f"layer_norm: elements of type {x.dtype} (bfloat16, float16 or float32)")
+    for t in (w, b):
+        if t is not None and (t.dtype != torch.float32 or t.shape != (c,) or not t.is_contiguous() or t.device != x.device):
+            raise ValueError(f"layer_norm: weight and bias are contiguous float32 tensors of {c} elements beside x")
+    return hip.LayerNormDesc(x=hip.ptr(x), w=hip.ptr(w), b=hip.ptr(b), stats=hip.ptr(stats), rows=rows, C=c, ldx=x.stride(0), dtype=hip.DTYPE[x.dtype],
+                             eps=eps, **more)
+
+
+def layer_norm_forward(x: Tensor, w: Optional[Tensor], b: Optional[Tensor], eps: float = 1e-5, *, want_stats: bool = True, out: Optional[Tensor] = None):
+    """Layer norm of every row of x [rows, C] (bf16, fp16 or fp32; rows any number of elements apart, e.g. a column slice); w, b: fp32
+    [C] or None.  Returns (y, stats fp32 [rows, 2] or None)."""
+    rows, c = x.shape
+    y = torch.empty(rows, c, device=x.device, dtype=x.dtype) if out is None else out
+    assert x.stride(1) == 1 and y.shape == x.shape and y.dtype == x.dtype and y.stride(1) == 1
+    stats = torch.empty(rows, 2, device=x.device, dtype=torch.float32) if want_stats else None
+    d = _ln_desc(x, w, b, stats, eps, y=hip.ptr(y), ldy=y.stride(0))
+    with hip.on_device_of(x):
+        _launch("ln_fwd_kernel", lambda: (_nb(x, y, w, b, stats), 8.0 * x.numel(), f"R{rows} C{c}"),
+                lambda: hip.call("ddpm_layer_norm_forward", C.byref(d), hip.stream()))
+    return y, stats
+
+
+def layer_norm_backward(x: Tensor, dy: Tensor, w: Optional[Tensor], stats: Tensor, *, want_dx: bool = True, want_dw: bool = True,
+                        want_db: bool = True):
+    """Gradients of layer_norm_forward: (dx like x or None, dw fp32 [C] or None, db fp32 [C] or None)."""
+    rows, c = x.shape
+    assert dy.shape == x.shape and dy.dtype == x.dtype and dy.stride(1) == 1 and x.stride(1) == 1
+    assert stats.shape == (rows, 2) and stats.dtype == torch.float32 and stats.is_contiguous()
+    dx = torch.empty(rows, c, device=x.device, dtype=x.dtype) if want_dx else None
+    dw = torch.empty(c, device=x.device, dtype=torch.float32) if want_dw else None
+    db = torch.empty(c, device=x.device, dtype=torch.float32) if want_db else None
+    d = _ln_desc(x, w, None, stats, 0.0, dy=hip.ptr(dy), lddy=dy.stride(0), dx=hip.ptr(dx), lddx=c, dw=hip.ptr(dw), db=hip.ptr(db))
+    part = None
+    if want_dw or want_db:
+        n = hip.lib().ddpm_layer_norm_part_rows(C.byref(d))
+        if n < 0:
+            hip.check(n, "layer_norm_backward")
+        part = torch.empty(n, 2, c, device=x.device, dtype=torch.float32)
+        d.part = hip.ptr(part)
+    with hip.on_device_of(x):
+        _launch("ln_bwd_kernel", lambda: (_nb(x, dy, dx, w, stats, dw, db), 12.0 * x.numel(), f"R{rows} C{c}"),
+                lambda: hip.call("ddpm_layer_norm_backward", C.byref(d), hip.stream()))
+    return dx, dw, db
+
+
+def grad_norm(grads, norm_type: float = 2.0, max_norm: Optional[float] = None) -> Tensor:
+    """Global norm (2 or infinity) of a list of gradients as a fp32 device scalar; with max_norm they are also clipped in place
+    (multiplied by min(1, max_norm / (norm + 1e-6))).  bf16, fp16 and fp32 tensors of any dense layout, on one device."""
+    import numpy as np
+    kinds = {2.0: hip.NORM_L2, float("inf"): hip.NORM_INF}
+    if float(norm_type) not in kinds:
+        raise ValueError(f"grad_norm: the 2-norm and the infinity norm are there, not norm_type={norm_type}")
+    if max_norm is not None and not max_norm >= 0:
+        raise ValueError(f"grad_norm: max_norm must not be negative, got {max_norm}")
+    dev = grads[0].device
+    if dev.type != "cuda":
+        raise RuntimeError("grad_norm runs on the HIP kernels only: gradients must live on an MI355X (cuda) device")
+    if {g.device for g in grads} != {dev}:
+        raise ValueError("grad_norm: all gradients must be on one device")
+    try:
+        size = np.array([hip.DTYPE[g.dtype] for g in grads], dtype=np.uint8)
+    except KeyError as e:
+        raise ValueError(f"grad_norm: gradients of type {e} (bfloat16, float16 or float32)") from None
+    for g in grads:
+        if not g.is_contiguous() and not (g.layout == torch.strided and torch.ops.aten.is_non_overlapping_and_dense(g)):
+            raise ValueError("grad_norm: a gradient has gaps or overlaps in its memory; make it contiguous first")
+    at = np.array([g.data_ptr() for g in grads], dtype=np.uint64)
+    n = np.array([g.numel() for g in grads], dtype=np.int64)
+    at, n, size = _merge_spans(at, n, size)
+    norm = torch.empty((), device=dev, dtype=torch.float32)
+    launch_grad_norm(at, n, size, kinds[float(norm_type)], max_norm, norm)
+    return norm
+
+
+def _merge_spans(at, n, kind):
+    """Spans of memory by address, empty ones left out, neighbours of one type joined, one that occurs twice counted once."""
+    import numpy as np
+    order = np.argsort(at, kind="stable")
+    order = order[n[order] > 0]
+    at, n, kind = at[order], n[order], kind[order]
+    if len(at) < 2:
+        return at, n, kind
+    same = (at[1:] == at[:-1]) & (n[1:] == n[:-1]) & (kind[1:] == kind[:-1])
+    if same.any():
+        keep = np.concatenate(([True], ~same))
+        at, n, kind = at[keep], n[keep], kind[keep]
+    end = at + (n * np.where(kind == hip.DTYPE[torch.float32], 4, 2)).astype(np.uint64)
+    if (at[1:] < end[:-1]).any():
+        raise ValueError("grad_norm: two gradients overlap in memory")
+    start = np.flatnonzero(np.concatenate(([True], (at[1:] != end[:-1]) | (kind[1:] != kind[:-1]))))
+    return at[start], np.add.reduceat(n, start), kind[start]
+
+
+def launch_grad_norm(at, n, kind, norm_type: int, max_norm: Optional[float], norm: Tensor) -> None:
+    """at, n, kind: host arrays (uint64 addresses, int64 element counts, uint8 types of hip.DTYPE) of spans on norm's device."""
+    lib, k = hip.lib(), len(at)
+    with hip.on_device_of(norm):
+        work = torch.empty(lib.ddpm_grad_norm_work_bytes(k, n.ctypes.data), device=norm.device, dtype=torch.uint8)
+        clip = max_norm is not None
+        _launch("grad_norm_kernel", lambda: (int((n * (2 + 2 * (kind == 2))).sum()) * (3 if clip else 1), 2.0 * int(n.sum()), f"{k} spans"),
+                lambda: hip.call("ddpm_grad_norm", at.ctypes.data, n.ctypes.data, kind.ctypes.data, k, norm_type, int(clip), max_norm if clip else 0.0,
+                                 hip.ptr(norm), hip.ptr(work), hip.stream()))
+
+
 def dwconv3x3(x: Tensor, w9c: Tensor, bias: Optional[Tensor], out: Optional[Tensor] = None, gn_part_groups: int = 0):
     """x: NHWC bf16; w9c: fp32 [9][C] tap-major.  gn_part_groups > 0: returns (y, part) with part = fp32 [N][groups][parts][2]
     partial sums (x, x^2) of y for gn_act_forward(stat_part=part), or None where the launch cannot deliver them."""

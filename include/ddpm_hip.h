@@ -564,6 +564,45 @@ typedef struct ddpm_sample_norm_desc {
 int ddpm_sample_norm_forward(const ddpm_sample_norm_desc* d, ddpm_stream_t stream);
 int ddpm_sample_norm_backward(const ddpm_sample_norm_desc* d, ddpm_stream_t stream);
 
+/* ---- layer norm over the last axis of token rows (layer_norm.hip) ------------------------------------------------
+ * y = (x - mean) * rstd * w + b per row of C elements, 1 <= C <= 8192; x, y, dy, dx have the element type `dtype`, rows ld*
+ * elements apart (ld* >= C; any value and any alignment of the element type: rows that are 16-byte aligned throughout are moved
+ * in 16-byte vectors, others element by element).  w, b: fp32 [C], NULL = 1 and 0.  stats: fp32 [rows][2] (mean, rstd), written
+ * by forward when not NULL, read by backward.  Backward: dx (NULL: not wanted) and dw, db fp32 [C] (each NULL: not wanted), written
+ * whole, also for rows = 0; they need part = fp32 [ddpm_layer_norm_part_rows(d)][2][C] (that call returns -1 for a bad descriptor).
+ * The sums' order is fixed: equal inputs give equal bits. */
+enum { DDPM_BF16 = 0, DDPM_F16 = 1, DDPM_F32 = 2 };
+typedef struct ddpm_layer_norm_desc {
+    const void* x; const void* dy;
+    void* y; void* dx;
+    const float* w; const float* b;
+    float* stats; float* part;
+    float* dw; float* db;
+    int64_t rows, ldx, ldy, lddy, lddx;
+    int32_t C, dtype;
+    float eps;
+} ddpm_layer_norm_desc;
+int ddpm_layer_norm_part_rows(const ddpm_layer_norm_desc* d);
+int ddpm_layer_norm_forward(const ddpm_layer_norm_desc* d, ddpm_stream_t stream);
+int ddpm_layer_norm_backward(const ddpm_layer_norm_desc* d, ddpm_stream_t stream);
+
+/* ---- global gradient norm over many tensors, and clipping (grad_clip.hip) ----------------------------------------
+ * norm = (sum over all elements of all tensors of g^2)^(1/2) for norm_type = DDPM_NORM_L2, max |g| for DDPM_NORM_INF (NaN if any
+ * element is NaN), rounded once to fp32.  Squares are summed in fp64 in a fixed order: no overflow for any finite gradients.
+ * The count tensors are described by three HOST arrays, read before the call returns: device address (aligned to the element
+ * type), number of elements, element type.  max_norm >= 0 with clip != 0: then every element is multiplied by
+ * min(1, max_norm / (norm + 1e-6)) in fp32 and rounded to its type, in place (NaN norm: all become NaN).  The tensors must not overlap.
+ * norm: fp32 device scalar.  work: ddpm_grad_norm_work_bytes(count, numel) bytes of device memory. */
+enum { DDPM_NORM_L2 = 0, DDPM_NORM_INF = 1 };
+int64_t ddpm_grad_norm_work_bytes(int count, const int64_t* numel);
+int ddpm_grad_norm(const uint64_t* ptr, const int64_t* numel, const uint8_t* dtype, int count, int norm_type, int clip, float max_norm,
+                   float* norm, void* work, ddpm_stream_t stream);
+/* ddpm_adam_step on clipped gradients, without a pass that clips them: norm = the device scalar of ddpm_grad_norm over the gradients,
+ * grad_scale multiplies both the gradients and their norm before max_norm is compared. */
+int ddpm_adam_step_clipped(float* p, const float* g, float* m, float* v, float* ema, int64_t n, const float* lr_dev, float lr,
+                           float beta1, float beta2, float eps, float weight_decay, float ema_decay, float grad_scale, int64_t* step,
+                           const float* norm, float max_norm, ddpm_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif
