@@ -1,7 +1,8 @@
 """Layers of a conditioning sequence's encoder (the tokens that ConditionalModule attends to): layer norm over the channels of each
-token, as autograd functions and modules on the HIP kernels.  They take tokens as rows, [..., C], in bf16, fp16 or fp32; parameters
-are fp32, as everywhere in this package.  The reference has no such encoder; its ConditionalModule takes the sequence from
-outside (constituent_blocks.py:402-437 there)."""
+token, and attention over packed sequences of different lengths (causal or not, grouped heads, learned relative position bias), as
+autograd functions and modules on the HIP kernels.  Activations are bf16, fp16 or (layer norm) fp32; parameters are fp32, as
+everywhere in this package.  The reference has no such encoder; its ConditionalModule takes the sequence from outside
+(constituent_blocks.py:402-437 there)."""
 from __future__ import annotations
 
 from typing import Optional
@@ -70,3 +71,84 @@ class LayerNorm(nn.Module):
         if x.shape[-1:] != self.normalized_shape:
             raise ValueError(f"LayerNorm({self.normalized_shape[0]}): last axis of {tuple(x.shape)}")
         return layer_norm(x, self.weight, self.bias, self.eps)
+
+
+# ---- attention over packed sequences ----------------------------------------------------------------------------------------
+def _heads(t: Tensor) -> Tensor:
+    """t [tokens, heads, width] as the kernels read it: contiguous heads, 16-byte aligned, no two on each other; copied where it is not"""
+    fits = t.stride(2) == 1 and t.data_ptr() % 16 == 0 and all(t.shape[i] <= 1 or (t.stride(i) >= t.shape[2] and t.stride(i) % 8 == 0) for i in (0, 1))
+    return t if fits else t.clone(memory_format=torch.contiguous_format)
+
+
+class _PackedAttentionFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, v, table, ends_q, ends_k, bucket_of, causal: bool, scale: Optional[float]):
+        q, k, v = _heads(q), _heads(k), _heads(v)
+        train = any(ctx.needs_input_grad)
+        o, lse, o32 = ops.packed_attention_forward(q, k, v, ends_q, ends_k, causal=causal, scale=scale, table=table, bucket_of=bucket_of,
+                                                   want_lse=train, want_o32=table is not None and ctx.needs_input_grad[3])
+        ctx.save_for_backward(q, k, v, table, ends_q, ends_k, bucket_of, o, lse, o32)
+        ctx.how = (causal, scale)
+        return o
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dout: Tensor):
+        q, k, v, table, ends_q, ends_k, bucket_of, o, lse, o32 = ctx.saved_tensors
+        dq, dk, dv, dtable = ops.packed_attention_backward(q, k, v, o, lse, _heads(dout), ends_q, ends_k, causal=ctx.how[0], scale=ctx.how[1], table=table,
+                                                           bucket_of=bucket_of, o32=o32, want_dtable=o32 is not None)
+        return dq, dk, dv, dtable, None, None, None, None, None
+
+
+def packed_attention(q: Tensor, k: Tensor, v: Tensor, ends: Tensor, *, ends_k: Optional[Tensor] = None, causal: bool = False,
+                     scale: Optional[float] = None, bias_table: Optional[Tensor] = None, bias_buckets: Optional[Tensor] = None) -> Tensor:
+    """softmax(scale q k^T + bias) v within each of several sequences that lie one behind the other.
+
+    q: [tokens, heads, width], k, v: [tokens, shared heads, width], bf16 or fp16; head h uses shared head h // (heads / shared heads).
+    width: a multiple of 8 up to 128; scale: 1 / sqrt(width) unless given (positive).  Views of a packed projection's output are read in
+    place; what the kernels cannot read in place (rows that are not contiguous or not 16-byte aligned) is copied first.
+    ends: int32 [sequences + 1] on the device, ascending from 0: sequence b is the rows ends[b] .. ends[b + 1] - 1 of q (and of k, v, unless
+    ends_k gives theirs).  Nothing is read back to the host, and no longest length is needed.  Rows outside of all sequences come out as zeros.
+    causal: a query sees the keys up to its own place, counted from the sequences' ends where there are more or fewer keys than queries.
+    A query that sees no key gets zeros.
+    bias_table [buckets, heads] (fp32, learned) with bias_buckets [2 far + 1] (int32, relative_position_buckets): adds
+    bias_table[bucket of (key's place - query's place), head] to the score.
+    Differentiable once in q, k, v and bias_table."""
+    for name, t in (("q", q), ("k", k), ("v", v)):
+        if t.dim() != 3:
+            raise ValueError(f"packed_attention: {name} of shape {tuple(t.shape)} is not [tokens, heads, width]")
+    _need_gpu("packed_attention", q, k, v, ends, ends_k, bias_table, bias_buckets)
+    return _PackedAttentionFn.apply(q, k, v, bias_table, ends, ends_k, bias_buckets, bool(causal), scale)
+
+
+def relative_position_buckets(num_buckets: int = 32, max_distance: int = 128, bidirectional: bool = True) -> Tensor:
+    """Bucket of every distance key - query from -far to far, int32 [2 far + 1] (what is further away shares the bucket at that end; far <=
+    max_distance is the first distance of the last bucket).  Half of the buckets (bidirectional: of each direction's half) hold one
+    distance each, e = 0, 1, ... of them; the other k have borders that grow geometrically, bucket e + t beginning at the first
+    distance n with (n / e)^k >= (max_distance / e)^t.  The borders are found in whole numbers, so that none depends on how a logarithm
+    is rounded.  Not bidirectional: keys behind the query share bucket 0."""
+    num_buckets, max_distance = int(num_buckets), int(max_distance)
+    side = num_buckets // 2 if bidirectional else num_buckets
+    e = side // 2
+    k = side - e
+    if e < 1 or num_buckets % (2 if bidirectional else 1) or not e < max_distance <= 1024:
+        raise ValueError(f"relative_position_buckets: {num_buckets} buckets for distances up to {max_distance} "
+                         f"(at least {4 if bidirectional else 2} buckets, an even number if bidirectional, distances over {max(e, 1)} and up to 1024)")
+    near = [n if n < e else e + min(k - 1, sum(n ** k * e ** t >= max_distance ** t * e ** k for t in range(1, k))) for n in range(max_distance + 1)]
+    far = max(4, next(n for n, b in enumerate(near) if b == near[-1]))
+    near = (near + [near[-1]] * far)[:far + 1]
+    ahead = [(side + b if bidirectional else 0) for b in near[1:]]
+    return torch.tensor(near[:0:-1] + near[:1] + ahead, dtype=torch.int32)
+
+
+class RelativePositionBias(nn.Module):
+    """A learned table of one bias per bucket and head, with the buckets of all distances: packed_attention(..., **bias()).  One of them
+    may serve every layer of an encoder; its gradient is the sum over the layers."""
+
+    def __init__(self, num_buckets: int, heads: int, max_distance: int = 128, bidirectional: bool = True, device=None):
+        super().__init__()
+        self.weight = nn.Parameter(torch.zeros(num_buckets, heads, device=device))
+        self.register_buffer("buckets", relative_position_buckets(num_buckets, max_distance, bidirectional).to(device), persistent=False)
+
+    def forward(self) -> dict:
+        return {"bias_table": self.weight, "bias_buckets": self.buckets}

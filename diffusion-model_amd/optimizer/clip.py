@@ -14,7 +14,7 @@ from ..runtime import ops
 def _grads(parameters: Union[Tensor, Iterable[Tensor]]) -> List[Tensor]:
     if isinstance(parameters, Tensor):
         parameters = [parameters]
-    return [p.grad for p in parameters if p.grad is not None]
+    return [g for p in parameters if (g := p.grad) is not None]
 
 
 @torch.no_grad()

@@ -91,6 +91,13 @@ class SampleNormDesc(C.Structure):
                 ("act_beta", _vp), ("dbeta_part", _vp)]
 
 
+class PackedAttnDesc(C.Structure):
+    _fields_ = [(k, _vp) for k in ("q", "k", "v", "o", "dout", "dq", "dk", "dv")] + [
+        (f"{k}_{s}", _i64) for k in ("q", "k", "v", "o", "dout", "dq", "dk", "dv") for s in ("row", "head")] + [
+        (k, _vp) for k in ("o32", "lse", "dsum", "ends_q", "ends_k", "table", "bucket_of", "dtable", "dtable_part")] + [
+        (k, C.c_int32) for k in ("Tq", "Tk", "B", "H", "Hk", "dh", "dtype", "causal", "zero_rest", "buckets", "far")] + [("scale", _f)]
+
+
 class LayerNormDesc(C.Structure):
     _fields_ = [(k, _vp) for k in ("x", "dy", "y", "dx", "w", "b", "stats", "part", "dw", "db")] + [
         (k, _i64) for k in ("rows", "ldx", "ldy", "lddy", "lddx")] + [("C", C.c_int32), ("dtype", C.c_int32), ("eps", _f)]
@@ -205,6 +212,9 @@ _PROTOS = {
     "ddpm_grad_norm_work_bytes": ([_i, _vp], _i64),
     "ddpm_grad_norm": ([_vp, _vp, _vp, _i, _i, _i, _f, _vp, _vp, _vp], _i),
     "ddpm_adam_step_clipped": ([_vp, _vp, _vp, _vp, _vp, _i64, _vp, _f, _f, _f, _f, _f, _f, _f, _vp, _vp, _f, _vp], _i),
+    "ddpm_packed_attn_slots": ([_i, _i], _i),
+    "ddpm_packed_attention_forward": ([C.POINTER(PackedAttnDesc), _vp], _i),
+    "ddpm_packed_attention_backward": ([C.POINTER(PackedAttnDesc), _vp], _i),
     "ddpm_dropout_masks": ([_vp, _vp, _i, _i64, _f, _vp, _vp], _i),
 }
 
@@ -242,7 +252,7 @@ def ptr(t):
 
 def stream() -> int:
     """The hipStream_t torch currently enqueues on (so launches are captured by torch.cuda graphs too)."""
-    return torch.cuda.current_stream().cuda_stream
+    return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device())      # (torch.cuda.current_stream() wraps it in an object: 2.7 us)
 
 
 def on_device_of(t):

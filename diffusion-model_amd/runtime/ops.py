@@ -509,6 +509,72 @@ def attention_backward(q: Tensor, k: Tensor, v: Tensor, o: Tensor, lse: Tensor, 
             lambda: hip.call("ddpm_attention_backward", C.byref(d), hip.stream()))
 
 
+def _packed_desc(q: Tensor, k: Tensor, v: Tensor, ends_q: Tensor, ends_k: Optional[Tensor], causal: bool, scale: Optional[float],
+                 table: Optional[Tensor], bucket_of: Optional[Tensor], zero_rest: bool) -> hip.PackedAttnDesc:
+    if q.dim() != 3 or k.dim() != 3 or k.shape != v.shape or q.shape[2] != k.shape[2] or q.shape[1] % max(1, k.shape[1]):
+        raise ValueError(f"packed_attention: q {tuple(q.shape)}, k {tuple(k.shape)}, v {tuple(v.shape)} are not [tokens, heads, width] with whole groups of heads")
+    if q.dtype not in (BF16, torch.float16) or k.dtype != q.dtype or v.dtype != q.dtype:
+        raise ValueError(f"packed_attention: q, k, v of types {q.dtype}, {k.dtype}, {v.dtype} (all bfloat16 or all float16)")
+    ek = ends_q if ends_k is None else ends_k
+    for e in (ends_q, ek):
+        if e.dtype != torch.int32 or e.dim() != 1 or e.numel() < 1 or not e.is_contiguous() or e.numel() != ends_q.numel() or e.device != q.device:
+            raise ValueError("packed_attention: the sequences' boundaries are contiguous int32 tensors of (sequences + 1) beside q")
+    if (table is None) != (bucket_of is None):
+        raise ValueError("packed_attention: the position bias needs both its table and the buckets of the distances")
+    d = hip.PackedAttnDesc(q=q.data_ptr(), k=k.data_ptr(), v=v.data_ptr(), q_row=q.stride(0), q_head=q.stride(1), k_row=k.stride(0), k_head=k.stride(1),
+                           v_row=v.stride(0), v_head=v.stride(1), ends_q=ends_q.data_ptr(), ends_k=ek.data_ptr(), Tq=q.shape[0], Tk=k.shape[0],
+                           B=ends_q.numel() - 1, H=q.shape[1], Hk=k.shape[1], dh=q.shape[2], dtype=hip.DTYPE[q.dtype], causal=int(causal),
+                           zero_rest=int(zero_rest), scale=q.shape[2] ** -0.5 if scale is None else scale)
+    if table is not None:
+        if table.dtype != torch.float32 or table.dim() != 2 or table.shape[1] != q.shape[1] or not table.is_contiguous() or table.device != q.device:
+            raise ValueError(f"packed_attention: the bias table is a contiguous float32 [buckets, {q.shape[1]}] tensor beside q, got {tuple(table.shape)} {table.dtype}")
+        if bucket_of.dtype != torch.int32 or bucket_of.dim() != 1 or bucket_of.numel() % 2 == 0 or not bucket_of.is_contiguous() or bucket_of.device != q.device:
+            raise ValueError("packed_attention: the buckets of the distances -far .. far are a contiguous int32 tensor of 2 far + 1 beside q")
+        d.table, d.bucket_of, d.buckets, d.far = table.data_ptr(), bucket_of.data_ptr(), table.shape[0], bucket_of.numel() // 2
+    return d
+
+
+def packed_attention_forward(q: Tensor, k: Tensor, v: Tensor, ends_q: Tensor, ends_k: Optional[Tensor] = None, *, causal: bool = False,
+                             scale: Optional[float] = None, table: Optional[Tensor] = None, bucket_of: Optional[Tensor] = None,
+                             out: Optional[Tensor] = None, want_lse: bool = True, want_o32: bool = False):
+    """Attention over packed sequences: q [Tq, H, width], k, v [Tk, Hk, width] (bf16 or fp16; slices of a packed projection are fine, with
+    strides that are multiples of 8), ends_q, ends_k int32 [sequences + 1].  Rows outside of all sequences: zeros in a new result, left
+    as they were in a given `out`.  Returns (o, lse fp32 [H, Tq] or None, o before rounding fp32 [Tq, H, width] or None)."""
+    d = _packed_desc(q, k, v, ends_q, ends_k, causal, scale, table, bucket_of, out is None)
+    o = torch.empty(q.shape, device=q.device, dtype=q.dtype) if out is None else out
+    assert o.shape == q.shape and o.dtype == q.dtype and o.stride(2) == 1 and q.stride(2) == 1 and k.stride(2) == 1 and v.stride(2) == 1
+    lse = torch.empty(q.shape[1], q.shape[0], device=q.device, dtype=torch.float32) if want_lse else None
+    o32 = torch.empty(q.shape, device=q.device, dtype=torch.float32) if want_o32 else None
+    d.o, d.o_row, d.o_head, d.lse, d.o32 = o.data_ptr(), o.stride(0), o.stride(1), hip.ptr(lse), hip.ptr(o32)
+    with hip.on_device_of(q):
+        # (the lengths are on the device: the probe's operation count takes every pair of one sequence)
+        _launch("pa_fwd_kernel", lambda: (_nb(q, k, v, o, lse, o32), 4.0 * q.numel() * k.shape[0], f"T{q.shape[0]} B{d.B} h{d.H}/{d.Hk} d{d.dh}"),
+                lambda: hip.call("ddpm_packed_attention_forward", C.byref(d), hip.stream()))
+    return o, lse, o32
+
+
+def packed_attention_backward(q: Tensor, k: Tensor, v: Tensor, o: Tensor, lse: Tensor, dout: Tensor, ends_q: Tensor, ends_k: Optional[Tensor] = None, *,
+                              causal: bool = False, scale: Optional[float] = None, table: Optional[Tensor] = None, bucket_of: Optional[Tensor] = None,
+                              o32: Optional[Tensor] = None, want_dtable: bool = False, grads=None):
+    """Gradients of packed_attention_forward: (dq, dk, dv, dtable fp32 or None).  grads = (dq, dk, dv) writes into those (any strides that are
+    multiples of 8) and leaves rows outside of all sequences; new ones are zero there.  want_dtable takes o32 from the forward pass."""
+    d = _packed_desc(q, k, v, ends_q, ends_k, causal, scale, table, bucket_of, grads is None)
+    dq, dk, dv = (torch.empty(t.shape, device=t.device, dtype=t.dtype) for t in (q, k, v)) if grads is None else grads
+    assert dout.shape == q.shape and dout.dtype == q.dtype and lse.shape == (q.shape[1], q.shape[0]) and lse.is_contiguous()
+    assert all(t.stride(2) == 1 for t in (q, k, v, o, dout, dq, dk, dv)) and (not want_dtable or o32 is not None)
+    dsum = torch.empty_like(lse)
+    dtable = torch.empty_like(table) if want_dtable else None
+    part = torch.empty(hip.lib().ddpm_packed_attn_slots(d.Tq, d.B) * d.H * d.buckets, device=q.device, dtype=torch.float32) if want_dtable else None
+    d.lse, d.dsum, d.o32, d.dtable, d.dtable_part = lse.data_ptr(), dsum.data_ptr(), hip.ptr(o32), hip.ptr(dtable), hip.ptr(part)
+    d.o, d.o_row, d.o_head, d.dout, d.dout_row, d.dout_head = o.data_ptr(), o.stride(0), o.stride(1), dout.data_ptr(), dout.stride(0), dout.stride(1)
+    d.dq, d.dq_row, d.dq_head, d.dk, d.dk_row, d.dk_head = dq.data_ptr(), dq.stride(0), dq.stride(1), dk.data_ptr(), dk.stride(0), dk.stride(1)
+    d.dv, d.dv_row, d.dv_head = dv.data_ptr(), dv.stride(0), dv.stride(1)
+    with hip.on_device_of(q):
+        _launch("pa_bwd_kernel", lambda: (_nb(q, k, v, o, dout, dq, dk, dv, lse, o32), 14.0 * q.numel() * k.shape[0], f"T{q.shape[0]} B{d.B} h{d.H}/{d.Hk} d{d.dh}"),
+                lambda: hip.call("ddpm_packed_attention_backward", C.byref(d), hip.stream()))
+    return dq, dk, dv, dtable
+
+
 def sample_norm_forward(a: Tensor, b: Optional[Tensor], act: int, gamma: Tensor, beta: Tensor, eps: float = 1e-5,
                         act_beta: Optional[Tensor] = None):
     """y = GroupNorm(1, C)(act(a) + b) over each sample of bf16 [N,S,1,C].  Returns (y, stats fp32 [N,2])."""
@@ -597,20 +663,23 @@ def grad_norm(grads, norm_type: float = 2.0, max_norm: Optional[float] = None) -
         raise ValueError(f"grad_norm: the 2-norm and the infinity norm are there, not norm_type={norm_type}")
     if max_norm is not None and not max_norm >= 0:
         raise ValueError(f"grad_norm: max_norm must not be negative, got {max_norm}")
-    dev = grads[0].device
-    if dev.type != "cuda":
+    # (hundreds of tensors: one pass of C-level calls for each property, not a Python loop over all of them)
+    index, count = set(map(Tensor.get_device, grads)), len(grads)
+    if -1 in index:
         raise RuntimeError("grad_norm runs on the HIP kernels only: gradients must live on an MI355X (cuda) device")
-    if {g.device for g in grads} != {dev}:
+    if len(index) > 1:
         raise ValueError("grad_norm: all gradients must be on one device")
+    dev = grads[0].device
     try:
-        size = np.array([hip.DTYPE[g.dtype] for g in grads], dtype=np.uint8)
+        size = np.fromiter((hip.DTYPE[g.dtype] for g in grads), np.uint8, count)
     except KeyError as e:
         raise ValueError(f"grad_norm: gradients of type {e} (bfloat16, float16 or float32)") from None
-    for g in grads:
-        if not g.is_contiguous() and not (g.layout == torch.strided and torch.ops.aten.is_non_overlapping_and_dense(g)):
-            raise ValueError("grad_norm: a gradient has gaps or overlaps in its memory; make it contiguous first")
-    at = np.array([g.data_ptr() for g in grads], dtype=np.uint64)
-    n = np.array([g.numel() for g in grads], dtype=np.int64)
+    if not all(map(Tensor.is_contiguous, grads)):
+        for g in grads:
+            if g.layout != torch.strided or not torch.ops.aten.is_non_overlapping_and_dense(g):
+                raise ValueError("grad_norm: a gradient has gaps or overlaps in its memory; make it contiguous first")
+    at = np.fromiter(map(Tensor.data_ptr, grads), np.uint64, count)
+    n = np.fromiter(map(Tensor.numel, grads), np.int64, count)
     at, n, size = _merge_spans(at, n, size)
     norm = torch.empty((), device=dev, dtype=torch.float32)
     launch_grad_norm(at, n, size, kinds[float(norm_type)], max_norm, norm)

@@ -603,6 +603,37 @@ int ddpm_adam_step_clipped(float* p, const float* g, float* m, float* v, float* 
                            float beta1, float beta2, float eps, float weight_decay, float ema_decay, float grad_scale, int64_t* step,
                            const float* norm, float max_norm, ddpm_stream_t stream);
 
+/* ---- attention over packed sequences, grouped heads, relative position bias (packed_attention.hip) -------------------
+ * Sequence b of B is the rows ends_q[b] .. ends_q[b+1]-1 of q, o, and ends_k[b] .. ends_k[b+1]-1 of k, v (int32 [B+1] on the device, ascending;
+ * they are read there and clamped to Tq, Tk rows, and may be the same array).  Per sequence and head: o = softmax(scale q k^T + bias) v, over all
+ * keys, or with causal != 0 over the keys j <= i + (its keys - its queries) for its query i.  A query that sees no key gets o = 0.
+ * Head h of H uses head h / (H / Hk) of k, v.  Element (row, head, d) of x is x[row * x_row + head * x_head + d], type `dtype` (DDPM_BF16 or
+ * DDPM_F16); strides are multiples of 8, base pointers 16-byte aligned, dh a multiple of 8 up to 128.
+ * Bias: table fp32 [buckets][H], bucket_of int32 [2 far + 1] (device): the bucket of the distance key - query (the query's place
+ * counted from the sequence's end when causal: i + keys - queries) clamped to -far .. far; 4 <= far <= 1024.  Both NULL: no bias.
+ * Rows outside of all sequences: zeros in o (dq, dk, dv) with zero_rest != 0, left as they were otherwise.
+ * lse fp32 [H][Tq] (base-2 log-sum-exp, -inf without a key) and o32 fp32 [Tq][H][dh] (o before rounding) are written by forward when
+ * not NULL (o32 of a launch with a bias is computed from probabilities in two 16-bit parts, i.e. to about 2^-16); backward reads lse, and
+ * o32 in place of o where it is given: dtable needs it, since o's own rounding would be its largest error.
+ * Backward writes dq, dk, dv (whole rows, any strides as above) and, when not NULL, dtable fp32 [buckets][H].  dsum: workspace fp32 [H][Tq];
+ * dtable_part: workspace fp32 [ddpm_packed_attn_slots(Tq, B)][H][buckets].  All sums have a fixed order: equal inputs, equal bits.
+ * An element of v (k in backward) that is not finite reaches the rows that see it, and may reach up to 63 earlier ones when causal. */
+typedef struct ddpm_packed_attn_desc {
+    const void* q; const void* k; const void* v; void* o;
+    const void* dout; void* dq; void* dk; void* dv;
+    int64_t q_row, q_head, k_row, k_head, v_row, v_head, o_row, o_head;
+    int64_t dout_row, dout_head, dq_row, dq_head, dk_row, dk_head, dv_row, dv_head;
+    float* o32; float* lse; float* dsum;
+    const int32_t* ends_q; const int32_t* ends_k;
+    const float* table; const int32_t* bucket_of;
+    float* dtable; float* dtable_part;
+    int32_t Tq, Tk, B, H, Hk, dh, dtype, causal, zero_rest, buckets, far;
+    float scale;
+} ddpm_packed_attn_desc;
+int ddpm_packed_attn_slots(int Tq, int B);
+int ddpm_packed_attention_forward(const ddpm_packed_attn_desc* d, ddpm_stream_t stream);
+int ddpm_packed_attention_backward(const ddpm_packed_attn_desc* d, ddpm_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif
