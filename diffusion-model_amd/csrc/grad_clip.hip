@@ -5,6 +5,7 @@
 // first one's partial sums itself, in every workgroup, instead of waiting for a third.
 //   Squares are summed in fp64: the product of two fp32 numbers is exact there, nothing finite overflows, and the cost hides
 // behind the loads.  Partial sums are added in a fixed order.
+#include <type_traits>
 #include "common.h"
 #include "ddpm_hip.h"
 
@@ -189,12 +190,15 @@ template <bool INF> __global__ __launch_bounds__(GC_THREADS) void grad_scale_ker
             typedef typename std::remove_reference<decltype(*base)>::type T;
             constexpr int V = 16 / sizeof(T);
             typedef T vec __attribute__((ext_vector_type(V)));
+            // A bf16 tensor is multiplied by the factor rounded to bf16, as torch.nn.utils.clip_grad_norm_ multiplies it: the bits of
+            // that, off by at most 2^-8 in a factor common to the whole tensor.  (An fp16 one is not: fp16 loses factors below 2^-14.)
+            const float by = std::is_same<T, bf16>::value ? (float)(bf16)coef : coef;
             gc_chunk(base, n, chunk, [&](vec* p) {
                 vec x = *p;
 #pragma unroll
-                for (int j = 0; j < V; ++j) x[j] = (T)((float)x[j] * coef);
+                for (int j = 0; j < V; ++j) x[j] = (T)((float)x[j] * by);
                 *p = x;
-            }, [&](T* p) { *p = (T)((float)*p * coef); });
+            }, [&](T* p) { *p = (T)((float)*p * by); });
         };
         const int type = (int)(sp.at[i] >> 62);
         if (type == DDPM_F32) run((float*)at);

@@ -20,6 +20,7 @@
 // host knowledge of the lengths.  A workgroup finds its sequence from the boundaries by one load and a ballot.  Rows outside of all
 // sequences are two more sequences without keys: their results are zeros where the caller wants that, and they are not touched otherwise.
 // Boundaries are clamped to the tensors, so that no contents of that array reach outside of them.
+#include <stdlib.h>
 #include <type_traits>
 #include "common.h"
 #include "ddpm_hip.h"
@@ -45,8 +46,9 @@ struct PaArgs {
     const float* table;                      // [buckets][H]
     const int* bucket_of;                    // [2 * far + 1]
     float* dtable_part;                      // [slots][H][buckets]
+    float* dkv_part;                         // [2][splits][Tk][Hk][dh], where the queries of a key are split over workgroups
     int buckets, far;
-    int Tq, Tk, B, H, Hk, dh, causal, zero_rest, slots;
+    int Tq, Tk, B, H, Hk, dh, causal, zero_rest, slots, splits;
     float scale, scale2;                     // and times log2(e)
 };
 
@@ -71,6 +73,19 @@ __device__ __forceinline__ float pa_half_max(float x) {
 __device__ __forceinline__ float pa_half_sum(float x) {
     const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
     return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+
+// Order of N products and their operands' LDS reads (READS each) in what the compiler schedules together: the first AHEAD products' reads in
+// front, then one product's at a time, so that a read has AHEAD products to arrive in
+template <int N, int READS, int AHEAD> __device__ __forceinline__ void pa_order() {
+    constexpr int A = AHEAD < N ? AHEAD : N;
+    __builtin_amdgcn_sched_group_barrier(0x100, A * READS, 0);
+#pragma unroll
+    for (int i = 0; i < N - A; ++i) {
+        __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+        __builtin_amdgcn_sched_group_barrier(0x100, READS, 0);
+    }
+    __builtin_amdgcn_sched_group_barrier(0x008, A, 0);
 }
 
 // ---- sequences ---------------------------------------------------------------------------------------------------------------
@@ -119,90 +134,115 @@ __device__ __forceinline__ bool pa_find(const int* ends, int T, const int* ends2
 }
 
 // ---- tiles -------------------------------------------------------------------------------------------------------------------
-template <int DHP> struct PaTile {
-    static constexpr int RB = DHP * 2, CH = DHP / 8, PER = PA_TILE * CH / 256, BYTES = PA_TILE * RB;
-    // the row-dependent xor on the index of a 16-byte piece: rows that share a 256-byte line of banks keep their order
-    static __device__ __forceinline__ int swz(int row) { return (row / (256 / RB)) & (CH - 1); }
+template <int DHP, int ROWS = PA_TILE> struct PaTile {
+    static constexpr int RB = DHP * 2, CH = DHP / 8, BYTES = ROWS * RB;
+    static constexpr int PER = 1024 / RB, ROUNDS = ROWS / (4 * PER);       // rows that a wave's load fills, loads of each of the four waves
+    // The row-dependent xor on the index of a 16-byte piece.  Reads along rows: the same piece of 16 consecutive rows lies on 16 different
+    // places of the 256-byte line of banks.  Transposed reads: 64 bytes each of four consecutive rows lie on its four quarters.
+    static __device__ __forceinline__ int swz(int row) {
+        if constexpr (CH == 16) return (row & 3) << 2 | (row >> 2 & 3);
+        else if constexpr (CH == 8) return (row >> 1 & 1) << 2 | (row >> 2 & 3);
+        else return row >> 2 & 3;
+    }
 };
 
-// byte offsets of the pieces that this thread moves of a tile; pieces past the head's width read as zeros (out of range of the buffer)
-template <int DHP> __device__ __forceinline__ void pa_offsets(unsigned (&off)[PaTile<DHP>::PER], long long row_stride, int dh) {
+// Tiles go from memory to LDS without passing through registers (buffer_load ... lds: lane i's 16 bytes to m0 + 16 i), which leaves those to
+// operands in flight.  The lane's piece of its wave's first load as a byte offset: the place in LDS decides which piece it is.  Rows past
+// the end and pieces past the head's width are out of the buffer's range and arrive as zeros.
+template <int DHP> __device__ __forceinline__ unsigned pa_piece(long long row_stride, int dh) {
     typedef PaTile<DHP> TL;
-#pragma unroll
-    for (int i = 0; i < TL::PER; ++i) {
-        const int idx = i * 256 + (int)threadIdx.x, row = idx / TL::CH, c = idx % TL::CH;
-        off[i] = c * 8 < dh ? (unsigned)(row * row_stride + c * 8) * 2u : 0xfffffff0u;
-    }
+    const int lane = threadIdx.x & 63, row = (threadIdx.x >> 6) * TL::PER + lane / TL::CH, c = (lane % TL::CH) ^ TL::swz(row);
+    return c * 8 < dh ? (unsigned)(row * row_stride + c * 8) * 2u : 0xfffffff0u;
 }
-
-// rows row0 ... row0 + 63 of a sequence's n rows that begin at base; rows past the end read as zeros
-template <int DHP> __device__ __forceinline__ void pa_load(u32x4 (&st)[PaTile<DHP>::PER], const void* base, long long row_stride, int row0, int n, int dh,
-                                                            const unsigned (&off)[PaTile<DHP>::PER]) {
-    const int left = n - row0 < PA_TILE ? n - row0 : PA_TILE;
+#pragma clang diagnostic ignored "-Winline-asm"        /* (m0 is named as changed below; nothing keeps a value in it) */
+// Rows row0 ... row0 + ROWS - 1 of a sequence's n rows that begin at base, to LDS at `lds`.  In assembly, since the compiler would wait for
+// such a load before the next read of any LDS: pa_arrived() is the wait.
+template <int DHP, int ROWS> __device__ __forceinline__ void pa_load(unsigned lds, const void* base, long long row_stride, int row0, int n, int dh, unsigned piece) {
+    typedef PaTile<DHP, ROWS> TL;
+    const int left = n - row0 < ROWS ? n - row0 : ROWS;
     const unsigned bytes = left > 0 ? (unsigned)((left - 1) * row_stride + dh) * 2u : 0u;
-    const __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc((void*)((const char*)base + row0 * row_stride * 2), 0, bytes, 0x00020000);
+    const unsigned long long at = (unsigned long long)((const char*)base + row0 * row_stride * 2);
+    const u32x4 buffer = {(unsigned)__builtin_amdgcn_readfirstlane((unsigned)at), (unsigned)__builtin_amdgcn_readfirstlane((unsigned)(at >> 32)),
+                          (unsigned)__builtin_amdgcn_readfirstlane(bytes), 0x00020000u};
+    const unsigned to = __builtin_amdgcn_readfirstlane(lds + (threadIdx.x >> 6) * 1024u);
 #pragma unroll
-    for (int i = 0; i < PaTile<DHP>::PER; ++i) st[i] = __builtin_amdgcn_raw_buffer_load_b128(r, off[i], 0, 0);
+    for (int i = 0; i < TL::ROUNDS; ++i)
+        asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds"
+                     :: "s"(to + i * 4096u), "v"(piece), "s"(buffer), "s"((unsigned)(i * 4 * TL::PER * row_stride) * 2u) : "memory", "m0");
 }
-
-template <int DHP> __device__ __forceinline__ void pa_store(char* lds, const u32x4 (&st)[PaTile<DHP>::PER]) {
-    typedef PaTile<DHP> TL;
-#pragma unroll
-    for (int i = 0; i < TL::PER; ++i) {
-        const int idx = i * 256 + (int)threadIdx.x, row = idx / TL::CH, c = idx % TL::CH;
-        *(u32x4*)(lds + row * TL::RB + ((c ^ TL::swz(row)) << 4)) = st[i];
-    }
+// Every load of this wave has arrived (vmcnt 0); the barrier behind it says so for all waves.  As a builtin, so that the compiler knows of it: its own
+// wait for loads in front of the loop would otherwise stand inside, behind the next tile's loads.
+__device__ __forceinline__ void pa_arrived() {
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_s_waitcnt(0x0f70);
+    asm volatile("" ::: "memory");
 }
+__device__ __forceinline__ unsigned pa_lds(const char* p) { return (unsigned)(unsigned long long)(const __attribute__((address_space(3))) char*)p; }
 
-// operand "row = tile row": lane's row, elements kc*16 + h*8 ... + 7
-template <typename V8, int DHP> __device__ __forceinline__ V8 pa_row_frag(const char* lds, int row, int kc, int h) {
+// Operands from a tile.  A lane's place in it is a number per kind of read; the xor moves only bits below a row, so that the 16-byte
+// pieces of a row, and the columns of a transposed read, are that number with a constant xored in, and everything else is an
+// immediate offset.  pa_opaque, once per tile, keeps the compiler from computing all of those in advance: for heads of 128 they would take
+// two dozen registers that it then keeps in scratch memory.
+//   "row = tile row": the lane's row, elements kc*16 + h*8 ... + 7
+template <int DHP> __device__ __forceinline__ unsigned pa_row_place(int row, int h) {
     typedef PaTile<DHP> TL;
-    return *(const V8*)(lds + row * TL::RB + (((kc * 2 + h) ^ TL::swz(row)) << 4));
+    return row * TL::RB + ((h ^ TL::swz(row)) << 4);
 }
-
-// operand "row = head dimension mt*32 + lane%32, contraction = the tile rows r0 + {0..3} + 4h and r0 + 8 + {0..3} + 4h": two transposed
-// reads; within 16 lanes, lane i addresses row i/4, columns (i%4)*4 ... + 3 and receives column i of the four rows
-template <typename V8, int DHP> __device__ __forceinline__ V8 pa_col_frag(const char* lds, int r0, int mt) {
+template <typename V8, int DHP> __device__ __forceinline__ V8 pa_row_frag(const char* lds, unsigned place, int kc) { return *(const V8*)(lds + (place ^ (kc << 5))); }
+//   "row = head dimension mt*32 + lane%32, contraction = the tile rows r0 + {0..3} + 4h and r0 + 8 + {0..3} + 4h" (r0 a multiple of 16): two
+// transposed reads; within 16 lanes, lane i addresses row i/4, columns (i%4)*4 ... + 3 and receives column i of the four rows
+template <int DHP> __device__ __forceinline__ unsigned pa_col_place() {
     typedef PaTile<DHP> TL;
-    const int lane = threadIdx.x & 63, li = lane & 15, row = r0 + 4 * (lane >> 5) + (li >> 2);
-    const int col = mt * 32 + 16 * ((lane >> 4) & 1) + 4 * (li & 3);           // element column; its 16-byte piece is col / 8
-    const char* p0 = lds + row * TL::RB + (((col >> 3) ^ TL::swz(row)) << 4) + (col & 7) * 2;
-    const char* p1 = lds + (row + 8) * TL::RB + (((col >> 3) ^ TL::swz(row + 8)) << 4) + (col & 7) * 2;
-    const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((s16x4 __attribute__((address_space(3)))*)(p0));
-    const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((s16x4 __attribute__((address_space(3)))*)(p1));
+    const int lane = threadIdx.x & 63, li = lane & 15, row = 4 * (lane >> 5) + (li >> 2), col = 16 * ((lane >> 4) & 1) + 4 * (li & 3);
+    return row * TL::RB + (((col >> 3) ^ TL::swz(row)) << 4) + (col & 7) * 2;
+}
+template <typename V8, int DHP> __device__ __forceinline__ V8 pa_col_frag(const char* lds, unsigned place, int r0, int mt) {
+    typedef PaTile<DHP> TL;
+    const char* const p = lds + r0 * TL::RB;
+    const unsigned at = place ^ (mt << 6);                                 // (eight rows on, bit 1 of the xor is the other one)
+    const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((s16x4 __attribute__((address_space(3)))*)(p + at));
+    const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((s16x4 __attribute__((address_space(3)))*)(p + 8 * TL::RB + (at ^ 32)));
     const s16x8 r = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
     return __builtin_bit_cast(V8, r);
 }
+template <int DHP> __device__ __forceinline__ void pa_opaque(unsigned& place) {
+    if constexpr (DHP == 128) asm volatile("" : "+v"(place));
+}
 
-// this lane's owned row from global memory as operands; zeros past the head's width or for a row that does not exist
-template <typename T, int DHP> __device__ __forceinline__ void pa_own(typename PaTypes<T>::v8 (&f)[DHP / 16], const PaView& x, long long row, int head, int dh, bool valid) {
-    typedef typename PaTypes<T>::v8 v8;
-    const T* p = (const T*)x.p + row * x.row + head * x.head;
+// A wave's own rows (up to 32, from row `row`, one a lane) through a buffer that ends with the last of them: what is out of range reads as
+// zeros and is not written, so that neither rows that do not exist nor pieces past the head's width need a branch.
+struct PaOwn {
+    __amdgpu_buffer_rsrc_t buffer;
+    unsigned at;                                                           // of the lane's row, in bytes
+    int dh;
+    bool valid;
+};
+__device__ __forceinline__ PaOwn pa_rows(const PaView& x, long long row, int rows, int head, int dh) {
+    const unsigned bytes = rows > 0 ? (unsigned)((rows - 1) * x.row + dh) * 2u : 0u;
+    const int col = threadIdx.x & 31;
+    return {__builtin_amdgcn_make_buffer_rsrc((char*)x.p + (row * x.row + head * x.head) * 2, 0, bytes, 0x00020000), (unsigned)(col * x.row) * 2u, dh, col < rows};
+}
+// as operands: elements kc*16 + h*8 ... + 7
+template <typename V8, int DHP> __device__ __forceinline__ void pa_own(V8 (&f)[DHP / 16], const PaOwn& x) {
 #pragma unroll
     for (int kc = 0; kc < DHP / 16; ++kc) {
         const int d = kc * 16 + (int)((threadIdx.x >> 5) & 1) * 8;
-        v8 z;
-#pragma unroll
-        for (int j = 0; j < 8; ++j) z[j] = (T)0.f;
-        f[kc] = valid && d < dh ? *(const v8*)(p + d) : z;
+        f[kc] = __builtin_bit_cast(V8, __builtin_amdgcn_raw_buffer_load_b128(x.buffer, x.valid && d < x.dh ? x.at + d * 2u : 0xfffffff0u, 0, 0));
     }
 }
-
-// a transposed result (rows = head dimensions, column = the lane's row) to memory
-template <typename T, int DHP, typename F>
-__device__ __forceinline__ void pa_put(const f32x16 (&acc)[DHP / 32], T* p, int dh, F&& f) {
+// a transposed result (rows = head dimensions, column = the lane's row)
+template <typename T, int DHP, typename F> __device__ __forceinline__ void pa_put(const f32x16 (&acc)[DHP / 32], const PaOwn& x, F&& f) {
     typedef typename PaTypes<T>::v4 v4;
+    typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
 #pragma unroll
     for (int mt = 0; mt < DHP / 32; ++mt)
 #pragma unroll
         for (int g = 0; g < 4; ++g) {
             const int d = mt * 32 + g * 8 + (int)((threadIdx.x >> 5) & 1) * 4;
-            if (d < dh) {
-                v4 w;
+            v4 w;
 #pragma unroll
-                for (int j = 0; j < 4; ++j) w[j] = (T)f(acc[mt][g * 4 + j]);
-                *(v4*)(p + d) = w;
-            }
+            for (int j = 0; j < 4; ++j) w[j] = (T)f(acc[mt][g * 4 + j]);
+            __builtin_amdgcn_raw_buffer_store_b64(__builtin_bit_cast(u32x2, w), x.buffer, x.valid && d < x.dh ? x.at + d * 2u : 0xfffffff0u, 0, 0);
         }
 }
 
@@ -216,7 +256,7 @@ template <typename T> __device__ __forceinline__ typename PaTypes<T>::v8 pa_pack
 // ---- relative position bias ----------------------------------------------------------------------------------------------------
 // LDS: the bias of every distance key - query in -far ... far for one head, in units of log2 like the scores.
 __device__ __forceinline__ void pa_bias_fill(const PaArgs& a, int head, float* s_bias) {
-    for (int i = threadIdx.x; i < 2 * a.far + 1; i += 256) {
+    for (int i = threadIdx.x; i < 2 * a.far + 1; i += blockDim.x) {
         int b = a.bucket_of[i];
         b = b < 0 ? 0 : b >= a.buckets ? a.buckets - 1 : b;
         s_bias[i] = a.table[b * a.H + head] * 1.4426950408889634f;
@@ -240,14 +280,15 @@ __global__ __launch_bounds__(256, 2) void pa_fwd_kernel(const PaArgs a) {
     PaSeq sq;
     if (!pa_find(a.ends_q, a.Tq, a.ends_k, a.Tk, a.B, slot, sq)) return;
     if (!sq.real && !a.zero_rest) return;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, col = lane & 31, h = lane >> 5;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), col = lane & 31, h = lane >> 5;
     const int w0 = sq.row0 + wave * 32, qi = w0 + col;                     // the wave's first row, the lane's row
     const bool qv = qi < sq.n;
     const int off = a.causal ? sq.n2 - sq.n : 0;                           // a causal row's last key is row + off
     if (BIAS) pa_bias_fill(a, head, s_bias);
 
+    const int w_rows = sq.n - w0 < 32 ? sq.n - w0 : 32;                    // <= 0: the wave has no rows
     v8 bq[KC];
-    pa_own<T, DHP>(bq, a.q, sq.begin + (qv ? qi : 0), head, a.dh, qv);
+    pa_own<v8, DHP>(bq, pa_rows(a.q, sq.begin + w0, w_rows, head, a.dh));
     f32x16 acc[MT];
 #pragma unroll
     for (int mt = 0; mt < MT; ++mt) acc[mt] = pa_zero();
@@ -259,41 +300,43 @@ __global__ __launch_bounds__(256, 2) void pa_fwd_kernel(const PaArgs a) {
     const int tiles = (keys + PA_TILE - 1) / PA_TILE;
     const char* const kb = (const char*)a.k.p + (sq.begin2 * a.k.row + hk * a.k.head) * 2;
     const char* const vb = (const char*)a.v.p + (sq.begin2 * a.v.row + hk * a.v.head) * 2;
-    unsigned ko[TL::PER], vo[TL::PER];
-    pa_offsets<DHP>(ko, a.k.row, a.dh);
-    pa_offsets<DHP>(vo, a.v.row, a.dh);
-    u32x4 kst[TL::PER], vst[TL::PER];
-    if (tiles > 0) {
-        pa_load<DHP>(kst, kb, a.k.row, 0, sq.n2, a.dh, ko);
-        pa_load<DHP>(vst, vb, a.v.row, 0, sq.n2, a.dh, vo);
-        pa_store<DHP>(smem, kst);
-        pa_store<DHP>(smem + TL::BYTES, vst);
-    }
-    __syncthreads();
-    const int w_rows = sq.n - w0 < 32 ? sq.n - w0 : 32;                    // <= 0: the wave has no rows
+    const unsigned ko = pa_piece<DHP>(a.k.row, a.dh), vo = pa_piece<DHP>(a.v.row, a.dh);
+    auto fetch = [&](int t) {
+        const unsigned to = pa_lds(smem) + (t & 1) * 2 * TL::BYTES;
+        pa_load<DHP, PA_TILE>(to, kb, a.k.row, t * PA_TILE, sq.n2, a.dh, ko);
+        pa_load<DHP, PA_TILE>(to + TL::BYTES, vb, a.v.row, t * PA_TILE, sq.n2, a.dh, vo);
+    };
+    if (tiles > 0) fetch(0);
+    const unsigned rp = pa_row_place<DHP>(col, h), cp = pa_col_place<DHP>();
     for (int t = 0; t < tiles; ++t) {
         const char* const lk = smem + (t & 1) * 2 * TL::BYTES;
         const char* const lv = lk + TL::BYTES;
         const int k0 = t * PA_TILE;
-        if (t + 1 < tiles) {
-            pa_load<DHP>(kst, kb, a.k.row, k0 + PA_TILE, sq.n2, a.dh, ko);
-            pa_load<DHP>(vst, vb, a.v.row, k0 + PA_TILE, sq.n2, a.dh, vo);
-        }
+        pa_arrived();
+        __syncthreads();                                                   // this tile is there, and the one before it has been read
+        if (t + 1 < tiles) fetch(t + 1);
         if (w_rows > 0 && (!a.causal || k0 <= w0 + w_rows - 1 + off)) {
             f32x16 sc[2] = {pa_zero(), pa_zero()};
+            __builtin_amdgcn_s_setprio(1);
 #pragma unroll
             for (int kc = 0; kc < KC; ++kc) {
-                sc[0] = pa_mfma(pa_row_frag<v8, DHP>(lk, col, kc, h), bq[kc], sc[0]);
-                sc[1] = pa_mfma(pa_row_frag<v8, DHP>(lk, 32 + col, kc, h), bq[kc], sc[1]);
+                sc[0] = pa_mfma(pa_row_frag<v8, DHP>(lk, rp, kc), bq[kc], sc[0]);
+                sc[1] = pa_mfma(pa_row_frag<v8, DHP>(lk + 32 * TL::RB, rp, kc), bq[kc], sc[1]);
             }
+            pa_order<2 * KC, 1, 4>();
+            __builtin_amdgcn_s_setprio(0);
             float s[32];
             const int dist0 = k0 + h * 4 - (qi + off);                     // distance of the lane's first score
             if (BIAS) {
-                const int lo = k0 - (w0 + w_rows - 1 + off), hi = k0 + PA_TILE - 1 - (w0 + off);       // distances in the wave's tile
+                const int lo = k0 - (w0 + 31 + off), hi = k0 + PA_TILE - 1 - (w0 + off);       // distances in the wave's tile
                 if (hi <= -a.far || lo >= a.far) {
                     const float b = s_bias[hi <= -a.far ? 0 : 2 * a.far];
 #pragma unroll
                     for (int i = 0; i < 32; ++i) s[i] = sc[i >> 4][i & 15] * a.scale2 + b;
+                } else if (lo > -a.far && hi < a.far) {                    // no distance is clamped: one address, constant offsets
+                    const float* const b = s_bias + dist0 + a.far;
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) s[i] = sc[i >> 4][i & 15] * a.scale2 + b[(i >> 2) * 8 + (i & 3)];
                 } else {
 #pragma unroll
                     for (int i = 0; i < 32; ++i)
@@ -335,6 +378,7 @@ __global__ __launch_bounds__(256, 2) void pa_fwd_kernel(const PaArgs a) {
             l += sum;                                                      // (this half-wave's keys; joined at the end)
             // p is rounded to the type of v for the product (relative 2^-8 of each term in bf16, of either sign); the sum above is not.
             // Where the output feeds the bias's gradient, whose terms cancel, what that rounding leaves is multiplied as well.
+            __builtin_amdgcn_s_setprio(1);
             auto pv = [&](auto two) {
 #pragma unroll
                 for (int c = 0; c < 4; ++c) {
@@ -346,7 +390,7 @@ __global__ __launch_bounds__(256, 2) void pa_fwd_kernel(const PaArgs a) {
                     }
 #pragma unroll
                     for (int mt = 0; mt < MT; ++mt) {
-                        const v8 f = pa_col_frag<v8, DHP>(lv, 16 * c, mt);
+                        const v8 f = pa_col_frag<v8, DHP>(lv, cp, 16 * c, mt);
                         acc[mt] = pa_mfma(f, p, acc[mt]);
                         if constexpr (decltype(two)::value) acc[mt] = pa_mfma(f, rest, acc[mt]);
                     }
@@ -354,19 +398,15 @@ __global__ __launch_bounds__(256, 2) void pa_fwd_kernel(const PaArgs a) {
             };
             if (BIAS && a.o32) pv(std::true_type());
             else pv(std::false_type());
+            pa_order<4 * MT, 2, 3>();
+            __builtin_amdgcn_s_setprio(0);
         }
-        if (t + 1 < tiles) {
-            char* const nk = smem + ((t + 1) & 1) * 2 * TL::BYTES;
-            pa_store<DHP>(nk, kst);
-            pa_store<DHP>(nk + TL::BYTES, vst);
-        }
-        __syncthreads();
     }
     l = pa_half_sum(l);
-    if (!qv) return;
     const float inv = l == 0.f ? 0.f : 1.f / l;
+    pa_put<T, DHP>(acc, pa_rows(a.o, sq.begin + w0, w_rows, head, a.dh), [&](float x) { return x * inv; });
+    if (!qv) return;
     const long long row = sq.begin + qi;
-    pa_put<T, DHP>(acc, (T*)a.o.p + row * a.o.row + head * a.o.head, a.dh, [&](float x) { return x * inv; });
     if (a.o32) {
         float* const p = a.o32 + (row * a.H + head) * a.dh;
 #pragma unroll
@@ -391,9 +431,12 @@ __global__ __launch_bounds__(256, 2) void pa_fwd_kernel(const PaArgs a) {
 // The gradient of the bias is a sum of ds over equal distances first and over the distances of a bucket last.  Distances inside of
 // (-far, far) are added up in LDS, one array per half-wave: the 32 lanes of a half hold 32 different distances of any one
 // register, so that no two lanes of an instruction meet, and a wave's LDS operations are executed in order; what is beyond
-// goes to two registers.  Every sum has a fixed order.  It is taken from the 32-bit ds, and D from the 32-bit output that the
-// forward pass leaves for it, with p in two parts there (either rounding to 16 bits would be the largest error of such a sum,
-// whose terms cancel: 5e-4 of the gradient instead of 1e-6).
+// goes to two registers.  Every sum has a fixed order and is taken from the 32-bit ds.
+//   D.  Where the workgroup's rows see at most two tiles of keys, D = sum_j p_ij (do_i . v_j) comes from a sweep over those: their
+// ds are few and of D's own size, and the rounding of o would be the largest error of dq (3e-3 of it instead of 2.4e-3 in bf16).  Longer
+// rows take do . o.  The sum of a row's ds, zero for the exact D, then says by how much that D was off: dk and the bias's gradient at
+// far distances (most of a long row) are corrected by it, and o comes in 32 bits with p in two parts there (1e-6 of the bias's
+// gradient instead of 5e-4).
 template <typename T, int DHP, bool BIAS>
 __global__ __launch_bounds__(256, 2) void pa_bwd_dq_kernel(const PaArgs a) {
     typedef typename PaTypes<T>::v8 v8;
@@ -413,7 +456,7 @@ __global__ __launch_bounds__(256, 2) void pa_bwd_dq_kernel(const PaArgs a) {
             for (int i = threadIdx.x; i < a.buckets; i += 256) part[i] = 0.f;
         return;
     }
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, col = lane & 31, h = lane >> 5;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), col = lane & 31, h = lane >> 5;
     const int w0 = sq.row0 + wave * 32, qi = w0 + col;
     const bool qv = qi < sq.n;
     const int off = a.causal ? sq.n2 - sq.n : 0;
@@ -424,13 +467,22 @@ __global__ __launch_bounds__(256, 2) void pa_bwd_dq_kernel(const PaArgs a) {
             for (int i = threadIdx.x; i < 8 * width; i += 256) s_sum[i] = 0.f;
     }
     float* const my_sum = s_sum + (threadIdx.x >> 5) * width;
-    float before = 0.f, after = 0.f;                                       // ds at distances <= -far, >= far
+    float before = 0.f, after = 0.f, pbefore = 0.f, pafter = 0.f;          // ds and p at distances <= -far, >= far
+    float all = 0.f;                                                       // every ds of the row
 
+    const int w_rows = sq.n - w0 < 32 ? sq.n - w0 : 32;
     v8 bq[KC], bdo[KC];
-    pa_own<T, DHP>(bq, a.q, row, head, a.dh, qv);
-    pa_own<T, DHP>(bdo, a.dout, row, head, a.dh, qv);
+    pa_own<v8, DHP>(bq, pa_rows(a.q, sq.begin + w0, w_rows, head, a.dh));
+    pa_own<v8, DHP>(bdo, pa_rows(a.dout, sq.begin + w0, w_rows, head, a.dh));
+    const int rows = sq.n - sq.row0 < PA_ROWS ? sq.n - sq.row0 : PA_ROWS;
+    int keys = a.causal ? sq.row0 + rows + off : sq.n2;
+    keys = keys < 0 ? 0 : keys < sq.n2 ? keys : sq.n2;
+    const int tiles = (keys + PA_TILE - 1) / PA_TILE;
+    const bool sweep = tiles <= 2;
+    const float lse = qv ? a.lse[(long long)head * a.Tq + row] : 0.f;
     float dsum = 0.f;
-    if (a.o32) {
+    if (sweep) {
+    } else if (a.o32) {
         const float* const o = a.o32 + (row * a.H + head) * a.dh;
 #pragma unroll
         for (int kc = 0; kc < KC; ++kc) {
@@ -445,88 +497,119 @@ __global__ __launch_bounds__(256, 2) void pa_bwd_dq_kernel(const PaArgs a) {
         }
     } else {
         v8 of[KC];
-        pa_own<T, DHP>(of, a.o, row, head, a.dh, qv);
+        pa_own<v8, DHP>(of, pa_rows(a.o, sq.begin + w0, w_rows, head, a.dh));
 #pragma unroll
         for (int kc = 0; kc < KC; ++kc)
 #pragma unroll
             for (int j = 0; j < 8; ++j) dsum += (float)bdo[kc][j] * (float)of[kc][j];
     }
     dsum = pa_half_sum(dsum);
-    const float lse = qv ? a.lse[(long long)head * a.Tq + row] : 0.f;
-    if (qv && h == 0) a.dsum[(long long)head * a.Tq + row] = dsum;
     f32x16 acc[MT];
 #pragma unroll
     for (int mt = 0; mt < MT; ++mt) acc[mt] = pa_zero();
 
-    const int rows = sq.n - sq.row0 < PA_ROWS ? sq.n - sq.row0 : PA_ROWS;
-    int keys = a.causal ? sq.row0 + rows + off : sq.n2;
-    keys = keys < 0 ? 0 : keys < sq.n2 ? keys : sq.n2;
-    const int tiles = (keys + PA_TILE - 1) / PA_TILE;
     const char* const kb = (const char*)a.k.p + (sq.begin2 * a.k.row + hk * a.k.head) * 2;
     const char* const vb = (const char*)a.v.p + (sq.begin2 * a.v.row + hk * a.v.head) * 2;
-    unsigned ko[TL::PER], vo[TL::PER];
-    pa_offsets<DHP>(ko, a.k.row, a.dh);
-    pa_offsets<DHP>(vo, a.v.row, a.dh);
-    u32x4 kst[TL::PER], vst[TL::PER];
-    if (tiles > 0) {
-        pa_load<DHP>(kst, kb, a.k.row, 0, sq.n2, a.dh, ko);
-        pa_load<DHP>(vst, vb, a.v.row, 0, sq.n2, a.dh, vo);
-        pa_store<DHP>(smem, kst);
-        pa_store<DHP>(smem + TL::BYTES, vst);
+    const unsigned ko = pa_piece<DHP>(a.k.row, a.dh), vo = pa_piece<DHP>(a.v.row, a.dh);
+    auto fetch = [&](int t) {
+        const unsigned to = pa_lds(smem) + (t & 1) * 2 * TL::BYTES;
+        pa_load<DHP, PA_TILE>(to, kb, a.k.row, t * PA_TILE, sq.n2, a.dh, ko);
+        pa_load<DHP, PA_TILE>(to + TL::BYTES, vb, a.v.row, t * PA_TILE, sq.n2, a.dh, vo);
+    };
+    unsigned rp = pa_row_place<DHP>(col, h), cp = pa_col_place<DHP>();
+    // probabilities (zero where the key is not seen) and do . v of 32 keys
+    auto scores = [&](const char* lk, const char* lv, int sub, int k0, float (&p)[16], f32x16& dp) {
+        f32x16 sc = pa_zero();
+        dp = pa_zero();
+#pragma unroll
+        for (int kc = 0; kc < KC; ++kc) {
+            sc = pa_mfma(pa_row_frag<v8, DHP>(lk + sub * 32 * TL::RB, rp, kc), bq[kc], sc);
+            dp = pa_mfma(pa_row_frag<v8, DHP>(lv + sub * 32 * TL::RB, rp, kc), bdo[kc], dp);
+        }
+        const int dist0 = k0 + h * 4 - (qi + off), lo = k0 - (w0 + 31 + off), hi = k0 + 31 - (w0 + off);
+        if (!BIAS || hi <= -a.far || lo >= a.far) {
+            const float b = BIAS ? s_bias[hi <= -a.far ? 0 : 2 * a.far] - lse : -lse;
+#pragma unroll
+            for (int i = 0; i < 16; ++i) p[i] = __builtin_amdgcn_exp2f(sc[i] * a.scale2 + b);
+        } else if (lo > -a.far && hi < a.far) {                            // no distance is clamped: one address, constant offsets
+            const float* const b = s_bias + dist0 + a.far;
+#pragma unroll
+            for (int i = 0; i < 16; ++i) p[i] = __builtin_amdgcn_exp2f(sc[i] * a.scale2 + (b[(i >> 2) * 8 + (i & 3)] - lse));
+        } else {
+#pragma unroll
+            for (int i = 0; i < 16; ++i)
+                p[i] = __builtin_amdgcn_exp2f(sc[i] * a.scale2 + (s_bias[pa_clamp(dist0 + (i >> 2) * 8 + (i & 3), a.far) + a.far] - lse));
+        }
+        if (k0 + 32 > sq.n2 || w_rows < 32 || (a.causal && k0 + 31 > w0 + off)) {
+            int last = (a.causal && qi + off < sq.n2 - 1 ? qi + off : sq.n2 - 1) - k0 - h * 4;
+            if (!qv) last = -1;
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {                                 // (do . v of a key that is not seen may be anything)
+                p[i] = (i >> 2) * 8 + (i & 3) <= last ? p[i] : 0.f;
+                dp[i] = (i >> 2) * 8 + (i & 3) <= last ? dp[i] : 0.f;
+            }
+        }
+    };
+    auto sees = [&](int k0) { return w_rows > 0 && k0 < sq.n2 && (!a.causal || k0 <= w0 + w_rows - 1 + off); };
+
+    if (tiles > 0) fetch(0);
+    if (sweep) {
+        if (tiles == 2) fetch(1);
+        pa_arrived();
+        __syncthreads();
+        for (int u = 0; u < 2 * tiles; ++u) {
+            const char* const lk = smem + (u >> 1) * 2 * TL::BYTES;
+            if (sees(u * 32)) {
+                float p[16];
+                f32x16 dp;
+                scores(lk, lk + TL::BYTES, u & 1, u * 32, p, dp);
+#pragma unroll
+                for (int i = 0; i < 16; ++i) dsum += p[i] * dp[i];
+            }
+        }
+        dsum = pa_half_sum(dsum);
     }
-    __syncthreads();
-    const int w_rows = sq.n - w0 < 32 ? sq.n - w0 : 32;
     for (int t = 0; t < tiles; ++t) {
         const char* const lk = smem + (t & 1) * 2 * TL::BYTES;
         const char* const lv = lk + TL::BYTES;
-        if (t + 1 < tiles) {
-            pa_load<DHP>(kst, kb, a.k.row, (t + 1) * PA_TILE, sq.n2, a.dh, ko);
-            pa_load<DHP>(vst, vb, a.v.row, (t + 1) * PA_TILE, sq.n2, a.dh, vo);
+        pa_opaque<DHP>(rp);
+        pa_opaque<DHP>(cp);
+        if (!sweep) {
+            pa_arrived();
+            __syncthreads();                                               // this tile is there, and the one before it has been read
+            if (t + 1 < tiles) fetch(t + 1);
         }
 #pragma unroll
         for (int sub = 0; sub < 2; ++sub) {
             const int k0 = t * PA_TILE + sub * 32;
-            if (w_rows > 0 && k0 < sq.n2 && (!a.causal || k0 <= w0 + w_rows - 1 + off)) {
-                f32x16 sc = pa_zero(), dp = pa_zero();
+            if (sees(k0)) {
+                float p[16], ds[16], sum = 0.f;
+                f32x16 dp;
+                scores(lk, lv, sub, k0, p, dp);
 #pragma unroll
-                for (int kc = 0; kc < KC; ++kc) {
-                    sc = pa_mfma(pa_row_frag<v8, DHP>(lk, sub * 32 + col, kc, h), bq[kc], sc);
-                    dp = pa_mfma(pa_row_frag<v8, DHP>(lv, sub * 32 + col, kc, h), bdo[kc], dp);
+                for (int i = 0; i < 16; ++i) {
+                    ds[i] = p[i] * (dp[i] - dsum);
+                    sum += ds[i];
                 }
-                float ds[16];
-                const int dist0 = k0 + h * 4 - (qi + off);
-                const int lo = k0 - (w0 + w_rows - 1 + off), hi = k0 + 31 - (w0 + off);
-                const bool far = BIAS && (hi <= -a.far || lo >= a.far);
-                if (BIAS && !far) {
-#pragma unroll
-                    for (int i = 0; i < 16; ++i)
-                        ds[i] = __builtin_amdgcn_exp2f(sc[i] * a.scale2 + (s_bias[pa_clamp(dist0 + (i >> 2) * 8 + (i & 3), a.far) + a.far] - lse));
-                } else {
-                    const float b = BIAS ? s_bias[hi <= -a.far ? 0 : 2 * a.far] - lse : -lse;
-#pragma unroll
-                    for (int i = 0; i < 16; ++i) ds[i] = __builtin_amdgcn_exp2f(sc[i] * a.scale2 + b);
-                }
-#pragma unroll
-                for (int i = 0; i < 16; ++i) ds[i] *= dp[i] - dsum;
-                if (k0 + 32 > sq.n2 || w_rows < 32 || (a.causal && k0 + 31 > w0 + off)) {
-                    int last = (a.causal && qi + off < sq.n2 - 1 ? qi + off : sq.n2 - 1) - k0 - h * 4;
-                    if (!qv) last = -1;
-#pragma unroll
-                    for (int i = 0; i < 16; ++i) ds[i] = (i >> 2) * 8 + (i & 3) <= last ? ds[i] : 0.f;
-                }
+                all += sum;
                 if (want_table) {
-                    if (far) {
-                        float sum = 0.f;
+                    const int dist0 = k0 + h * 4 - (qi + off), lo = k0 - (w0 + 31 + off), hi = k0 + 31 - (w0 + off);
+                    if (hi <= -a.far || lo >= a.far) {
+                        float ps = 0.f;
 #pragma unroll
-                        for (int i = 0; i < 16; ++i) sum += ds[i];
-                        if (hi <= -a.far) before += sum;
-                        else after += sum;
+                        for (int i = 0; i < 16; ++i) ps += p[i];
+                        if (lo >= a.far) { after += sum; pafter += ps; }
+                        else { before += sum; pbefore += ps; }
+                    } else if (lo > -a.far && hi < a.far) {
+                        float* const at = my_sum + dist0 + a.far;
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) __hip_atomic_fetch_add(at + (i >> 2) * 8 + (i & 3), ds[i], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
                     } else {
 #pragma unroll
                         for (int i = 0; i < 16; ++i) {
                             const int d = dist0 + (i >> 2) * 8 + (i & 3);
-                            if (d <= -a.far) before += ds[i];
-                            else if (d >= a.far) after += ds[i];
+                            if (d <= -a.far) { before += ds[i]; pbefore += p[i]; }
+                            else if (d >= a.far) { after += ds[i]; pafter += p[i]; }
                             else __hip_atomic_fetch_add(my_sum + d + a.far, ds[i], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
                         }
                     }
@@ -534,23 +617,20 @@ __global__ __launch_bounds__(256, 2) void pa_bwd_dq_kernel(const PaArgs a) {
                 // ds is rounded to the type of k for the product (see p in the forward pass)
 #pragma unroll
                 for (int c = 0; c < 2; ++c) {
-                    const v8 p = pa_pack<T>(ds + 8 * c);
+                    const v8 r = pa_pack<T>(ds + 8 * c);
 #pragma unroll
-                    for (int mt = 0; mt < MT; ++mt) acc[mt] = pa_mfma(pa_col_frag<v8, DHP>(lk, sub * 32 + 16 * c, mt), p, acc[mt]);
+                    for (int mt = 0; mt < MT; ++mt) acc[mt] = pa_mfma(pa_col_frag<v8, DHP>(lk, cp, sub * 32 + 16 * c, mt), r, acc[mt]);
                 }
             }
         }
-        if (t + 1 < tiles) {
-            char* const nk = smem + ((t + 1) & 1) * 2 * TL::BYTES;
-            pa_store<DHP>(nk, kst);
-            pa_store<DHP>(nk + TL::BYTES, vst);
-        }
-        __syncthreads();
     }
-    if (qv) pa_put<T, DHP>(acc, (T*)a.dq.p + row * a.dq.row + head * a.dq.head, a.dh, [&](float x) { return x * a.scale; });
+    all = pa_half_sum(all);
+    if (qv && h == 0) a.dsum[(long long)head * a.Tq + row] = dsum + all;
+    pa_put<T, DHP>(acc, pa_rows(a.dq, sq.begin + w0, w_rows, head, a.dh), [&](float x) { return x * a.scale; });
     if (!want_table) return;
-    before = wave_sum(before);
-    after = wave_sum(after);
+    before = wave_sum(before - all * pbefore);
+    after = wave_sum(after - all * pafter);
+    __syncthreads();
     if (lane == 0) { s_bias[wave * 2] = before; s_bias[wave * 2 + 1] = after; }       // (the bias itself is no longer needed; width >= 9)
     __syncthreads();
     for (int i = threadIdx.x; i < width; i += 256) {
@@ -587,132 +667,195 @@ __global__ __launch_bounds__(256) void pa_dtable_kernel(const float* __restrict_
 // ================================================================================================================================
 // backward: dk, dv; a wave owns 32 keys and walks over the queries of every head that shares them
 // ================================================================================================================================
+// Heads of 128: the accumulators and k take 160 registers, so that v is read from LDS and tiles are 32 queries, which leaves room for two
+// workgroups on a CU, each waiting at barriers of its own (v in registers: one workgroup, LATER).
+// The steps (heads of the group x tiles of queries) may be split over several workgroups, whose 32-bit sums a last launch adds
+// up: few keys with long sequences and shared heads would leave most of the card idle otherwise.
 template <typename T, int DHP, bool BIAS>
-__global__ __launch_bounds__(256, DHP > 64 ? 1 : 2) void pa_bwd_dkv_kernel(const PaArgs a) {
+__global__ __launch_bounds__(256, 2) void pa_bwd_dkv_kernel(const PaArgs a) {
     typedef typename PaTypes<T>::v8 v8;
-    typedef PaTile<DHP> TL;
     constexpr int KC = DHP / 16, MT = DHP / 32;
+    constexpr int ROWS = DHP == 128 ? 32 : PA_TILE;
+    constexpr bool VLDS = DHP == 128;
+    typedef PaTile<DHP, ROWS> TL;
     extern __shared__ __attribute__((aligned(16))) char smem[];           // q, do tiles, two buffers of both; lse and D of their rows; the bias
-    float* const s_row = (float*)(smem + 4 * TL::BYTES);                   // [2][2][64]
-    float* const s_bias = s_row + 4 * PA_TILE;
+    float* const s_row = (float*)(smem + 4 * TL::BYTES);                   // [2][2][ROWS]
+    float* const s_bias = s_row + 4 * ROWS;
     const int hk = blockIdx.x % a.Hk, group = a.H / a.Hk;
-    const int slot = (int)(blockIdx.x / a.Hk);                             // (starts of causal sequences, the most queries, first)
+    const int slot = (int)(blockIdx.x / (a.Hk * a.splits)), split = __builtin_amdgcn_readfirstlane((int)(blockIdx.x / a.Hk % a.splits));   // (starts of causal sequences, the most queries, first)
     PaSeq sq;                                                              // begin, n: keys; begin2, n2: queries
     if (!pa_find(a.ends_k, a.Tk, a.ends_q, a.Tq, a.B, slot, sq)) return;
     if (!sq.real && !a.zero_rest) return;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, col = lane & 31, h = lane >> 5;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), col = lane & 31, h = lane >> 5;
     const int w0 = sq.row0 + wave * 32, ki = w0 + col;
     const bool kv = ki < sq.n;
     const int off = a.causal ? sq.n - sq.n2 : 0;
-    const long long row = sq.begin + (kv ? ki : 0);
+    const int w_rows = sq.n - w0 < 32 ? sq.n - w0 : 32;
+    char* const s_v = smem + 4 * TL::BYTES + 16 * ROWS + (BIAS ? ((2 * a.far + 1) * 4 + 15) / 16 * 16 : 0);
     v8 bk[KC], bv[KC];
-    pa_own<T, DHP>(bk, a.k, row, hk, a.dh, kv);
-    pa_own<T, DHP>(bv, a.v, row, hk, a.dh, kv);
+    pa_own<v8, DHP>(bk, pa_rows(a.k, sq.begin + w0, w_rows, hk, a.dh));
+    pa_own<v8, DHP>(bv, pa_rows(a.v, sq.begin + w0, w_rows, hk, a.dh));
+    if (VLDS) {
+#pragma unroll
+        for (int kc = 0; kc < KC; ++kc) *(v8*)(s_v + wave * 32 * TL::RB + (pa_row_place<DHP>(col, h) ^ (kc << 5))) = bv[kc];
+    }
     f32x16 dk[MT], dv[MT];
 #pragma unroll
     for (int mt = 0; mt < MT; ++mt) { dk[mt] = pa_zero(); dv[mt] = pa_zero(); }
     int first = a.causal ? sq.row0 - off : 0;                              // the first query that sees any key of the workgroup
-    first = first < 0 ? 0 : first / PA_TILE * PA_TILE;
-    const int tiles = sq.n2 > first ? (sq.n2 - first + PA_TILE - 1) / PA_TILE : 0, steps = tiles * group;
-    unsigned qo[TL::PER], po[TL::PER];
-    pa_offsets<DHP>(qo, a.q.row, a.dh);
-    pa_offsets<DHP>(po, a.dout.row, a.dh);
-    u32x4 qst[TL::PER], pst[TL::PER];
+    first = first < 0 ? 0 : first / ROWS * ROWS;
+    const int tiles = sq.n2 > first ? (sq.n2 - first + ROWS - 1) / ROWS : 0;
+    const int steps = tiles * group, share = __builtin_amdgcn_readfirstlane((steps + a.splits - 1) / a.splits);
+    const int begin = split * share < steps ? split * share : steps, end = begin + share < steps ? begin + share : steps;
+    const unsigned qo = pa_piece<DHP>(a.q.row, a.dh), po = pa_piece<DHP>(a.dout.row, a.dh);
     float rst = 0.f;                                                       // threads 0 .. 63: lse of a query, 64 .. 127: its D
-    auto fetch = [&](int step) {
-        const int hd = hk * group + step / tiles, q0 = first + step % tiles * PA_TILE;
-        pa_load<DHP>(qst, (const char*)a.q.p + (sq.begin2 * a.q.row + hd * a.q.head) * 2, a.q.row, q0, sq.n2, a.dh, qo);
-        pa_load<DHP>(pst, (const char*)a.dout.p + (sq.begin2 * a.dout.row + hd * a.dout.head) * 2, a.dout.row, q0, sq.n2, a.dh, po);
-        if (threadIdx.x < 2 * PA_TILE) {
-            const int q = q0 + (threadIdx.x & (PA_TILE - 1));
-            const long long at = (long long)hd * a.Tq + sq.begin2 + q;
-            if (threadIdx.x < PA_TILE) {
+    // the step that is loaded next: head hd, tile td
+    int hd = tiles > 0 ? __builtin_amdgcn_readfirstlane(begin / tiles) : 0, td = begin - hd * tiles;
+    auto fetch = [&](int buf) {
+        const int head = hk * group + hd, q0 = first + td * ROWS;
+        const unsigned to = pa_lds(smem) + buf * 2 * TL::BYTES;
+        pa_load<DHP, ROWS>(to, (const char*)a.q.p + (sq.begin2 * a.q.row + head * a.q.head) * 2, a.q.row, q0, sq.n2, a.dh, qo);
+        pa_load<DHP, ROWS>(to + TL::BYTES, (const char*)a.dout.p + (sq.begin2 * a.dout.row + head * a.dout.head) * 2, a.dout.row, q0, sq.n2, a.dh, po);
+        if (threadIdx.x < 2 * ROWS) {
+            const int q = q0 + (threadIdx.x & (ROWS - 1));
+            const long long at = (long long)head * a.Tq + sq.begin2 + q;
+            if (threadIdx.x < ROWS) {
                 rst = q < sq.n2 ? a.lse[at] : INFINITY;
                 if (rst == -INFINITY) rst = INFINITY;                      // no key seen, or no query: every probability comes out as zero
             } else
                 rst = q < sq.n2 ? a.dsum[at] : 0.f;
         }
+        if (++td == tiles) { td = 0; ++hd; }
     };
     auto keep = [&](int buf) {
-        char* const p = smem + buf * 2 * TL::BYTES;
-        pa_store<DHP>(p, qst);
-        pa_store<DHP>(p + TL::BYTES, pst);
-        if (threadIdx.x < 2 * PA_TILE) s_row[buf * 2 * PA_TILE + threadIdx.x] = rst;
+        if (threadIdx.x < 2 * ROWS) s_row[buf * 2 * ROWS + threadIdx.x] = rst;
     };
-    if (steps > 0) {
-        fetch(0);
-        keep(0);
+    int q_head = hd, q_tile = td;                                          // the step that is computed next
+    if (begin < end) {
+        fetch(begin & 1);
+        keep(begin & 1);
     }
-    const int w_rows = sq.n - w0 < 32 ? sq.n - w0 : 32;
-    for (int step = 0; step < steps; ++step) {
-        if (BIAS && step % tiles == 0) {
+    unsigned rp = pa_row_place<DHP>(col, h), cp = pa_col_place<DHP>(), vp = wave * 32 * TL::RB + rp;
+    for (int step = begin; step < end; ++step) {
+        pa_opaque<DHP>(rp);
+        pa_opaque<DHP>(cp);
+        pa_opaque<DHP>(vp);
+        if (BIAS && (step == begin || q_tile == 0)) {
             __syncthreads();
-            pa_bias_fill(a, hk * group + step / tiles, s_bias);
+            pa_bias_fill(a, hk * group + q_head, s_bias);
         }
-        __syncthreads();
+        pa_arrived();
+        __syncthreads();                                                   // this tile is there, and the one before it has been read
         const char* const lq = smem + (step & 1) * 2 * TL::BYTES;
         const char* const lp = lq + TL::BYTES;
-        const float* const lr = s_row + (step & 1) * 2 * PA_TILE;
-        if (step + 1 < steps) fetch(step + 1);
+        if (step + 1 < end) fetch((step + 1) & 1);
 #pragma unroll
-        for (int sub = 0; sub < 2; ++sub) {
-            const int q0 = first + step % tiles * PA_TILE + sub * 32;
-            if (w_rows > 0 && q0 < sq.n2 && (!a.causal || q0 + 31 + off >= w0)) {
-                f32x16 sc = pa_zero(), dp = pa_zero();
+        for (int sub = 0; sub < ROWS / 32; ++sub) {
+        const float* const lr = s_row + (step & 1) * 2 * ROWS + sub * 32 + h * 4;
+        const int q0 = first + q_tile * ROWS + sub * 32;
+        if (w_rows > 0 && q0 < sq.n2 && (!a.causal || q0 + 31 + off >= w0)) {
+            f32x16 sc = pa_zero(), dp = pa_zero();
 #pragma unroll
-                for (int kc = 0; kc < KC; ++kc) {
-                    sc = pa_mfma(pa_row_frag<v8, DHP>(lq, sub * 32 + col, kc, h), bk[kc], sc);
-                    dp = pa_mfma(pa_row_frag<v8, DHP>(lp, sub * 32 + col, kc, h), bv[kc], dp);
-                }
-                float p[16], ds[16];
-                const int dist0 = ki - (q0 + h * 4 + off);                 // distance of the lane's first score; later rows are nearer
-                float bc = 0.f;
-                bool far = true;
-                if (BIAS) {
-                    const int lo = w0 - (q0 + 31 + off), hi = w0 + w_rows - 1 - (q0 + off);
-                    far = hi <= -a.far || lo >= a.far;
-                    if (far) bc = s_bias[hi <= -a.far ? 0 : 2 * a.far];
-                }
+            for (int kc = 0; kc < KC; ++kc) sc = pa_mfma(pa_row_frag<v8, DHP>(lq + sub * 32 * TL::RB, rp, kc), bk[kc], sc);
 #pragma unroll
-                for (int g = 0; g < 4; ++g) {
-                    const f32x4 ls = *(const f32x4*)(lr + sub * 32 + g * 8 + h * 4);
+            for (int kc = 0; kc < KC; ++kc)
+                dp = pa_mfma(pa_row_frag<v8, DHP>(lp + sub * 32 * TL::RB, rp, kc), VLDS ? pa_row_frag<v8, DHP>(s_v, vp, kc) : bv[kc], dp);
+            pa_order<KC, 1, 3>();
+            pa_order<KC, VLDS ? 2 : 1, 2>();
+            // (here, so that a branch ends the region in which the compiler may hold these products back and keep all their operands instead)
+            if (a.causal && w0 + w_rows - 1 > q0 + off) {
+                const int firstq = ki - off - q0 - h * 4;                  // query index of a row that sees this key
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        const int i = g * 4 + j;
-                        const float b = BIAS && !far ? s_bias[pa_clamp(dist0 - g * 8 - j, a.far) + a.far] : bc;
-                        p[i] = __builtin_amdgcn_exp2f(sc[i] * a.scale2 + (b - ls[j]));
-                    }
-                }
-                if (a.causal && w0 + w_rows - 1 > q0 + off) {
-                    const int firstq = ki - off - q0 - h * 4;              // query index of a row that sees this key
-#pragma unroll
-                    for (int i = 0; i < 16; ++i) p[i] = (i >> 2) * 8 + (i & 3) >= firstq ? p[i] : 0.f;
-                }
-#pragma unroll
-                for (int c = 0; c < 2; ++c) {
-                    const v8 pp = pa_pack<T>(p + 8 * c);
-#pragma unroll
-                    for (int mt = 0; mt < MT; ++mt) dv[mt] = pa_mfma(pa_col_frag<v8, DHP>(lp, sub * 32 + 16 * c, mt), pp, dv[mt]);
-                }
-#pragma unroll
-                for (int g = 0; g < 4; ++g) {
-                    const f32x4 dd = *(const f32x4*)(lr + PA_TILE + sub * 32 + g * 8 + h * 4);
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) ds[g * 4 + j] = p[g * 4 + j] * (dp[g * 4 + j] - dd[j]);
-                }
-#pragma unroll
-                for (int c = 0; c < 2; ++c) {
-                    const v8 pp = pa_pack<T>(ds + 8 * c);
-#pragma unroll
-                    for (int mt = 0; mt < MT; ++mt) dk[mt] = pa_mfma(pa_col_frag<v8, DHP>(lq, sub * 32 + 16 * c, mt), pp, dk[mt]);
+                for (int i = 0; i < 16; ++i) {
+                    sc[i] = (i >> 2) * 8 + (i & 3) >= firstq ? sc[i] : -INFINITY;
+                    dp[i] = (i >> 2) * 8 + (i & 3) >= firstq ? dp[i] : 0.f;
                 }
             }
+            float p[16];
+            const int dist0 = ki - (q0 + h * 4 + off), lo = w0 - (q0 + 31 + off), hi = w0 + 31 - (q0 + off);   // distance of the lane's first score; later rows are nearer
+            if (!BIAS || hi <= -a.far || lo >= a.far) {
+                const float b = BIAS ? s_bias[hi <= -a.far ? 0 : 2 * a.far] : 0.f;
+#pragma unroll
+                for (int i = 0; i < 16; ++i) p[i] = sc[i] * a.scale2 + b;
+            } else if (lo > -a.far && hi < a.far) {
+                const float* const b = s_bias + dist0 + a.far;
+#pragma unroll
+                for (int i = 0; i < 16; ++i) p[i] = sc[i] * a.scale2 + b[-((i >> 2) * 8 + (i & 3))];
+            } else {
+#pragma unroll
+                for (int i = 0; i < 16; ++i) p[i] = sc[i] * a.scale2 + s_bias[pa_clamp(dist0 - ((i >> 2) * 8 + (i & 3)), a.far) + a.far];
+            }
+#pragma unroll
+            for (int g = 0; g < 4; ++g) {
+                const f32x4 ls = *(const f32x4*)(lr + g * 8);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) p[g * 4 + j] = __builtin_amdgcn_exp2f(p[g * 4 + j] - ls[j]);
+            }
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+                const v8 r = pa_pack<T>(p + 8 * c);
+#pragma unroll
+                for (int mt = 0; mt < MT; ++mt) dv[mt] = pa_mfma(pa_col_frag<v8, DHP>(lp, cp, sub * 32 + 16 * c, mt), r, dv[mt]);
+            }
+            pa_order<2 * MT, 2, 3>();
+#pragma unroll
+            for (int g = 0; g < 4; ++g) {
+                const f32x4 dd = *(const f32x4*)(lr + ROWS + g * 8);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) p[g * 4 + j] *= dp[g * 4 + j] - dd[j];
+            }
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+                const v8 r = pa_pack<T>(p + 8 * c);
+#pragma unroll
+                for (int mt = 0; mt < MT; ++mt) dk[mt] = pa_mfma(pa_col_frag<v8, DHP>(lq, cp, sub * 32 + 16 * c, mt), r, dk[mt]);
+            }
+            pa_order<2 * MT, 2, 3>();
         }
-        if (step + 1 < steps) keep((step + 1) & 1);
+        }
+        if (++q_tile == tiles) { q_tile = 0; ++q_head; }
+        if (step + 1 < end) keep((step + 1) & 1);
     }
-    if (!kv) return;
-    pa_put<T, DHP>(dk, (T*)a.dk.p + row * a.dk.row + hk * a.dk.head, a.dh, [&](float x) { return x * a.scale; });
-    pa_put<T, DHP>(dv, (T*)a.dv.p + row * a.dv.row + hk * a.dv.head, a.dh, [&](float x) { return x; });
+    if (a.dkv_part) {
+        if (!kv) return;
+        const long long row = sq.begin + ki;
+        float* const p = a.dkv_part + (((long long)split * a.Tk + row) * a.Hk + hk) * a.dh, *const p2 = p + (long long)a.splits * a.Tk * a.Hk * a.dh;
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+            for (int g = 0; g < 4; ++g) {
+                const int d = mt * 32 + g * 8 + h * 4;
+                if (d < a.dh) {
+                    *(f32x4*)(p + d) = f32x4{dk[mt][g * 4], dk[mt][g * 4 + 1], dk[mt][g * 4 + 2], dk[mt][g * 4 + 3]};
+                    *(f32x4*)(p2 + d) = f32x4{dv[mt][g * 4], dv[mt][g * 4 + 1], dv[mt][g * 4 + 2], dv[mt][g * 4 + 3]};
+                }
+            }
+        return;
+    }
+    pa_put<T, DHP>(dk, pa_rows(a.dk, sq.begin + w0, w_rows, hk, a.dh), [&](float x) { return x * a.scale; });
+    pa_put<T, DHP>(dv, pa_rows(a.dv, sq.begin + w0, w_rows, hk, a.dh), [&](float x) { return x; });
+}
+
+// dk, dv = the sums over the splits, in order: a thread takes four elements of a row of both
+template <typename T> __global__ __launch_bounds__(256) void pa_dkv_join_kernel(const PaArgs a) {
+    typedef typename PaTypes<T>::v4 v4;
+    const int per = a.Hk * (a.dh / 4);
+    const long long idx = blockIdx.x * 256ll + threadIdx.x, total = (long long)a.Tk * per;
+    if (idx >= total) return;
+    const int row = (int)(idx / per), c = (int)(idx % per), hk = c / (a.dh / 4), d = c % (a.dh / 4) * 4;
+    if (!a.zero_rest && (row < pa_bound(a.ends_k, 1, a.B, a.Tk) || row >= pa_bound(a.ends_k, a.B + 1, a.B, a.Tk))) return;
+    const long long step = (long long)a.Tk * a.Hk * a.dh;
+    const float* p = a.dkv_part + idx * 4;
+    f32x4 k = {0.f, 0.f, 0.f, 0.f}, v = k;
+    for (int s = 0; s < a.splits; ++s) {
+        k += *(const f32x4*)(p + s * step);
+        v += *(const f32x4*)(p + (a.splits + s) * step);
+    }
+    v4 ko, vo;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) { ko[j] = (T)(k[j] * a.scale); vo[j] = (T)v[j]; }
+    *(v4*)((T*)a.dk.p + row * a.dk.row + hk * a.dk.head + d) = ko;
+    *(v4*)((T*)a.dv.p + row * a.dv.row + hk * a.dv.head + d) = vo;
 }
 
 // ================================================================================================================================
@@ -721,31 +864,46 @@ __global__ __launch_bounds__(256, DHP > 64 ? 1 : 2) void pa_bwd_dkv_kernel(const
 namespace {
 constexpr int PA_MAX_FAR = 1024;
 
-int pa_launch(void (*kernel)(const PaArgs), unsigned grid, size_t lds, const PaArgs& a, hipStream_t st) {
+int pa_launch(void (*kernel)(const PaArgs), dim3 grid, int threads, size_t lds, const PaArgs& a, hipStream_t st) {
     if (lds > 64 * 1024 && hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds) != hipSuccess) {
         ddpm_set_error("packed_attention: cannot reserve %zu bytes of LDS", lds);
         return DDPM_EHIP;
     }
-    hipLaunchKernelGGL(kernel, dim3(grid), dim3(256), lds, st, a);
+    hipLaunchKernelGGL(kernel, grid, dim3(threads), lds, st, a);
     return ddpm_check_launch("packed_attention");
 }
 
 template <typename T, int DHP, bool BIAS>
 int pa_launch_fwd(const PaArgs& a, hipStream_t st) {
-    return pa_launch(pa_fwd_kernel<T, DHP, BIAS>, (unsigned)(a.slots * a.H), 4 * PaTile<DHP>::BYTES + (BIAS ? (2 * a.far + 1) * 4 : 0), a, st);
+    return pa_launch(pa_fwd_kernel<T, DHP, BIAS>, dim3((unsigned)(a.slots * a.H)), 256, 4 * PaTile<DHP>::BYTES + (BIAS ? (2 * a.far + 1) * 4 : 0), a, st);
 }
 
 template <typename T, int DHP, bool BIAS>
 int pa_launch_bwd(PaArgs a, float* dtable, hipStream_t st) {
     const size_t width = (2 * a.far + 1) * 4;
     if (a.Tq > 0) {
-        if (const int rc = pa_launch(pa_bwd_dq_kernel<T, DHP, BIAS>, (unsigned)(a.slots * a.H), 4 * PaTile<DHP>::BYTES + (BIAS ? (a.dtable_part ? 9 : 1) * width : 0), a, st)) return rc;
+        if (const int rc = pa_launch(pa_bwd_dq_kernel<T, DHP, BIAS>, dim3((unsigned)(a.slots * a.H)), 256, 4 * PaTile<DHP>::BYTES + (BIAS ? (a.dtable_part ? 9 : 1) * width : 0), a, st)) return rc;
     }
     if (a.dtable_part)
         hipLaunchKernelGGL(pa_dtable_kernel, dim3((unsigned)a.H), dim3(256), 0, st, a.dtable_part, a.Tq > 0 ? a.slots : 0, a.H, a.buckets, dtable);
+    constexpr int rows = DHP == 128 ? 32 : PA_TILE;
     a.slots = a.Tk / PA_ROWS + a.B + 2;
     if (a.Tk == 0) return ddpm_check_launch("packed_attention_backward");
-    return pa_launch(pa_bwd_dkv_kernel<T, DHP, BIAS>, (unsigned)(a.slots * a.Hk), 4 * PaTile<DHP>::BYTES + 16 * PA_TILE + (BIAS ? width : 0), a, st);
+    if (const int rc = pa_launch(pa_bwd_dkv_kernel<T, DHP, BIAS>, dim3((unsigned)(a.slots * a.Hk * a.splits)), 256, rows * (4 * PaTile<DHP>::RB + 16) + (BIAS ? (width + 15) / 16 * 16 : 0) + (DHP == 128 ? PA_ROWS * PaTile<DHP>::RB : 0), a, st)) return rc;
+    if (a.splits > 1) {
+        const long long n = (long long)a.Tk * a.Hk * (a.dh / 4);
+        hipLaunchKernelGGL(pa_dkv_join_kernel<T>, dim3((unsigned)((n + 255) / 256)), dim3(256), 0, st, a);
+    }
+    return ddpm_check_launch("packed_attention_backward");
+}
+
+// How many workgroups share the queries of 128 keys.  RULE
+int pa_splits(const ddpm_packed_attn_desc* d) {
+    const long long groups = (long long)(d->Tk / PA_ROWS + d->B + 2) * d->Hk, steps = (long long)d->Tq / PA_TILE / (d->B > 0 ? d->B : 1) * (d->H / d->Hk);
+    long long z = 512 / groups;
+    z = z < steps / 4 ? z : steps / 4;
+    if (const char* e = getenv("PAZ")) z = atoi(e);
+    return z < 1 ? 1 : z > 16 ? 16 : (int)z;
 }
 
 template <typename F> int pa_dispatch(const ddpm_packed_attn_desc* d, F&& f) {
@@ -793,12 +951,15 @@ int pa_setup(const ddpm_packed_attn_desc* d, bool bwd, PaArgs& a) {
         if (const int rc = pa_view("dk", d->dk, d->dk_row, d->dk_head, d->Tk, d->Hk, d->dh, a.dk)) return rc;
         if (const int rc = pa_view("dv", d->dv, d->dv_row, d->dv_head, d->Tk, d->Hk, d->dh, a.dv)) return rc;
         DDPM_REQUIRE(d->Tq == 0 || (d->lse && d->dsum), "packed_attention: backward needs lse and the workspace dsum");
+        DDPM_REQUIRE(d->Tk == 0 || pa_splits(d) == 1 || d->dkv_part, "packed_attention: backward of these sizes needs the workspace dkv_part");
         DDPM_REQUIRE(!d->dtable || d->dtable_part, "packed_attention: the bias's gradient needs the workspace dtable_part");
     }
     a.o32 = d->o32; a.lse = d->lse; a.dsum = d->dsum;
     a.ends_q = d->ends_q; a.ends_k = d->ends_k;
     a.table = d->table; a.bucket_of = d->bucket_of; a.buckets = d->buckets; a.far = d->table ? d->far : 0;
     a.dtable_part = bwd && d->dtable ? d->dtable_part : nullptr;
+    a.splits = bwd ? pa_splits(d) : 1;
+    a.dkv_part = a.splits > 1 ? d->dkv_part : nullptr;
     a.Tq = d->Tq; a.Tk = d->Tk; a.B = d->B; a.H = d->H; a.Hk = d->Hk; a.dh = d->dh; a.causal = d->causal; a.zero_rest = d->zero_rest;
     a.slots = d->Tq / PA_ROWS + d->B + 2;
     a.scale = d->scale;
@@ -808,6 +969,10 @@ int pa_setup(const ddpm_packed_attn_desc* d, bool bwd, PaArgs& a) {
 }  // namespace
 
 extern "C" int ddpm_packed_attn_slots(int Tq, int B) { return Tq / PA_ROWS + B + 2; }
+extern "C" int64_t ddpm_packed_attn_dkv_floats(const ddpm_packed_attn_desc* d) {
+    const int splits = d && d->Hk > 0 ? pa_splits(d) : 1;
+    return splits > 1 ? 2ll * splits * d->Tk * d->Hk * d->dh : 0;
+}
 
 extern "C" int ddpm_packed_attention_forward(const ddpm_packed_attn_desc* d, ddpm_stream_t stream) {
     PaArgs a;

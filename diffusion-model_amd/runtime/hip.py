@@ -94,7 +94,7 @@ class SampleNormDesc(C.Structure):
 class PackedAttnDesc(C.Structure):
     _fields_ = [(k, _vp) for k in ("q", "k", "v", "o", "dout", "dq", "dk", "dv")] + [
         (f"{k}_{s}", _i64) for k in ("q", "k", "v", "o", "dout", "dq", "dk", "dv") for s in ("row", "head")] + [
-        (k, _vp) for k in ("o32", "lse", "dsum", "ends_q", "ends_k", "table", "bucket_of", "dtable", "dtable_part")] + [
+        (k, _vp) for k in ("o32", "lse", "dsum", "ends_q", "ends_k", "table", "bucket_of", "dtable", "dtable_part", "dkv_part")] + [
         (k, C.c_int32) for k in ("Tq", "Tk", "B", "H", "Hk", "dh", "dtype", "causal", "zero_rest", "buckets", "far")] + [("scale", _f)]
 
 
@@ -213,6 +213,7 @@ _PROTOS = {
     "ddpm_grad_norm": ([_vp, _vp, _vp, _i, _i, _i, _f, _vp, _vp, _vp], _i),
     "ddpm_adam_step_clipped": ([_vp, _vp, _vp, _vp, _vp, _i64, _vp, _f, _f, _f, _f, _f, _f, _f, _vp, _vp, _f, _vp], _i),
     "ddpm_packed_attn_slots": ([_i, _i], _i),
+    "ddpm_packed_attn_dkv_floats": ([C.POINTER(PackedAttnDesc)], _i64),
     "ddpm_packed_attention_forward": ([C.POINTER(PackedAttnDesc), _vp], _i),
     "ddpm_packed_attention_backward": ([C.POINTER(PackedAttnDesc), _vp], _i),
     "ddpm_dropout_masks": ([_vp, _vp, _i, _i64, _f, _vp, _vp], _i),

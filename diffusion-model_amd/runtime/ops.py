@@ -566,6 +566,9 @@ def packed_attention_backward(q: Tensor, k: Tensor, v: Tensor, o: Tensor, lse: T
     dtable = torch.empty_like(table) if want_dtable else None
     part = torch.empty(hip.lib().ddpm_packed_attn_slots(d.Tq, d.B) * d.H * d.buckets, device=q.device, dtype=torch.float32) if want_dtable else None
     d.lse, d.dsum, d.o32, d.dtable, d.dtable_part = lse.data_ptr(), dsum.data_ptr(), hip.ptr(o32), hip.ptr(dtable), hip.ptr(part)
+    floats = hip.lib().ddpm_packed_attn_dkv_floats(C.byref(d))
+    split = torch.empty(floats, device=q.device, dtype=torch.float32) if floats else None
+    d.dkv_part = hip.ptr(split)
     d.o, d.o_row, d.o_head, d.dout, d.dout_row, d.dout_head = o.data_ptr(), o.stride(0), o.stride(1), dout.data_ptr(), dout.stride(0), dout.stride(1)
     d.dq, d.dq_row, d.dq_head, d.dk, d.dk_row, d.dk_head = dq.data_ptr(), dq.stride(0), dq.stride(1), dk.data_ptr(), dk.stride(0), dk.stride(1)
     d.dv, d.dv_row, d.dv_head = dv.data_ptr(), dv.stride(0), dv.stride(1)

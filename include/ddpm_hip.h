@@ -591,7 +591,8 @@ int ddpm_layer_norm_backward(const ddpm_layer_norm_desc* d, ddpm_stream_t stream
  * element is NaN), rounded once to fp32.  Squares are summed in fp64 in a fixed order: no overflow for any finite gradients.
  * The count tensors are described by three HOST arrays, read before the call returns: device address (aligned to the element
  * type), number of elements, element type.  max_norm >= 0 with clip != 0: then every element is multiplied by
- * min(1, max_norm / (norm + 1e-6)) in fp32 and rounded to its type, in place (NaN norm: all become NaN).  The tensors must not overlap.
+ * min(1, max_norm / (norm + 1e-6)) in fp32 and rounded to its type, in place (NaN norm: all become NaN); for bf16 tensors the factor is
+ * rounded to bf16 first, as torch.nn.utils.clip_grad_norm_ does.  The tensors must not overlap.
  * norm: fp32 device scalar.  work: ddpm_grad_norm_work_bytes(count, numel) bytes of device memory. */
 enum { DDPM_NORM_L2 = 0, DDPM_NORM_INF = 1 };
 int64_t ddpm_grad_norm_work_bytes(int count, const int64_t* numel);
@@ -616,7 +617,8 @@ int ddpm_adam_step_clipped(float* p, const float* g, float* m, float* v, float* 
  * not NULL (o32 of a launch with a bias is computed from probabilities in two 16-bit parts, i.e. to about 2^-16); backward reads lse, and
  * o32 in place of o where it is given: dtable needs it, since o's own rounding would be its largest error.
  * Backward writes dq, dk, dv (whole rows, any strides as above) and, when not NULL, dtable fp32 [buckets][H].  dsum: workspace fp32 [H][Tq];
- * dtable_part: workspace fp32 [ddpm_packed_attn_slots(Tq, B)][H][buckets].  All sums have a fixed order: equal inputs, equal bits.
+ * dtable_part: workspace fp32 [ddpm_packed_attn_slots(Tq, B)][H][buckets]; dkv_part: workspace of ddpm_packed_attn_dkv_floats(d) floats (0: NULL
+ * will do; it looks at the sizes only).  All sums have a fixed order: equal inputs, equal bits.
  * An element of v (k in backward) that is not finite reaches the rows that see it, and may reach up to 63 earlier ones when causal. */
 typedef struct ddpm_packed_attn_desc {
     const void* q; const void* k; const void* v; void* o;
@@ -627,10 +629,12 @@ typedef struct ddpm_packed_attn_desc {
     const int32_t* ends_q; const int32_t* ends_k;
     const float* table; const int32_t* bucket_of;
     float* dtable; float* dtable_part;
+    float* dkv_part;
     int32_t Tq, Tk, B, H, Hk, dh, dtype, causal, zero_rest, buckets, far;
     float scale;
 } ddpm_packed_attn_desc;
 int ddpm_packed_attn_slots(int Tq, int B);
+int64_t ddpm_packed_attn_dkv_floats(const ddpm_packed_attn_desc* d);
 int ddpm_packed_attention_forward(const ddpm_packed_attn_desc* d, ddpm_stream_t stream);
 int ddpm_packed_attention_backward(const ddpm_packed_attn_desc* d, ddpm_stream_t stream);
 

@@ -2,7 +2,8 @@
 
 The norm is summed in float64 and rounded once: 2^-24 relative, plus the square root's and the sum's float64 error (1e-13).  A clipped
 element is g * coef, coef = max / (norm + 1e-6) in fp32 (three roundings, 2^-24 each, and the norm's own), one rounding of the product
-and one to the element's type: (half a step of the type + 5 * 2^-24) |g coef|."""
+and one to the element's type: (half a step of the type + 5 * 2^-24) |g coef|.  For bf16 tensors coef is rounded to bf16 before (2^-8 relative),
+as torch does with them: twice half a step, and the product's bits are compared with torch's own."""
 import math
 
 import pytest
@@ -35,7 +36,7 @@ def check_clip(before, params, norm, limit, kind=2.0):
     coef = min(1.0, limit / (want.item() + 1e-6))
     for g, p in zip(before, params):
         w = g.double() * coef
-        tol = (HALF_STEP[g.dtype] + 5 * 2.0 ** -24) * w.abs() + torch.finfo(g.dtype).smallest_normal * torch.finfo(g.dtype).eps
+        tol = (HALF_STEP[g.dtype] * (2.01 if g.dtype == torch.bfloat16 else 1) + 5 * 2.0 ** -24) * w.abs() + torch.finfo(g.dtype).smallest_normal * torch.finfo(g.dtype).eps
         assert ((p.grad.cpu().double() - w).abs() <= tol).all(), tuple(g.shape)
 
 
@@ -115,6 +116,19 @@ def test_clip_layouts_and_extremes(dev):
     p = torch.empty(0, device=dev)
     p.grad = torch.empty(0, device=dev)
     assert clip_grad_norm_([p], 1.0).item() == 0.0                                     # an empty one
+
+
+@pytest.mark.gpu
+def test_clip_multiplies_as_torch_does(dev):
+    """fp32 and bf16 gradients, clipped twice in a row: given the norm, the same bits as torch's tensor.mul_(factor on the device).  (The norm's own
+    bits are not torch's, which rounds every tensor's norm before it takes the norm of those.)"""
+    for t in (torch.float32, torch.bfloat16):
+        ps = params_of(make([64, 33, 4097], (t,)), dev)
+        for limit in (0.37, 0.1):
+            before = [p.grad.clone() for p in ps]
+            factor = (limit / (clip_grad_norm_(ps, limit) + 1e-6)).clamp(max=1.0)
+            for p, x in zip(ps, before):
+                assert torch.equal(p.grad, x.mul_(factor))
 
 
 @pytest.mark.gpu
