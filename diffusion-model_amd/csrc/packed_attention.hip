@@ -20,7 +20,6 @@
 // host knowledge of the lengths.  A workgroup finds its sequence from the boundaries by one load and a ballot.  Rows outside of all
 // sequences are two more sequences without keys: their results are zeros where the caller wants that, and they are not touched otherwise.
 // Boundaries are clamped to the tensors, so that no contents of that array reach outside of them.
-#include <stdlib.h>
 #include <type_traits>
 #include "common.h"
 #include "ddpm_hip.h"
@@ -73,6 +72,12 @@ __device__ __forceinline__ float pa_half_max(float x) {
 __device__ __forceinline__ float pa_half_sum(float x) {
     const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
     return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+
+// A wave's LDS operations are executed in order; the compiler keeps to it here, where lanes read what others wrote
+__device__ __forceinline__ void pa_wave_order() {
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_wave_barrier();
 }
 
 // Order of N products and their operands' LDS reads (READS each) in what the compiler schedules together: the first AHEAD products' reads in
@@ -428,10 +433,10 @@ __global__ __launch_bounds__(256, 2) void pa_fwd_kernel(const PaArgs a) {
 // ================================================================================================================================
 // backward: dq (and D, and the bias's gradient); a wave owns 32 queries
 // ================================================================================================================================
-// The gradient of the bias is a sum of ds over equal distances first and over the distances of a bucket last.  Distances inside of
-// (-far, far) are added up in LDS, one array per half-wave: the 32 lanes of a half hold 32 different distances of any one
-// register, so that no two lanes of an instruction meet, and a wave's LDS operations are executed in order; what is beyond
-// goes to two registers.  Every sum has a fixed order and is taken from the 32-bit ds.
+// The gradient of the bias is a sum of ds over equal distances first and over the distances of a bucket last.  A tile wholly at
+// distances beyond -far or far adds to two registers.  Of other tiles, 16 keys at a time go to LDS and come back by diagonals, a lane to
+// each, whose sums a wave adds to an array of its own (1.5 us of a workgroup's time for a tile's 16 registers as LDS atomics, which is
+// what fp32 ones cost; this way 0.1).  Every sum has a fixed order and is taken from the 32-bit ds.
 //   D.  Where the workgroup's rows see at most two tiles of keys, D = sum_j p_ij (do_i . v_j) comes from a sweep over those: their
 // ds are few and of D's own size, and the rounding of o would be the largest error of dq (3e-3 of it instead of 2.4e-3 in bf16).  Longer
 // rows take do . o.  The sum of a row's ds, zero for the exact D, then says by how much that D was off: dk and the bias's gradient at
@@ -445,7 +450,7 @@ __global__ __launch_bounds__(256, 2) void pa_bwd_dq_kernel(const PaArgs a) {
     extern __shared__ __attribute__((aligned(16))) char smem[];           // k, v tiles, two buffers of both; then the bias and its sums
     const int width = 2 * a.far + 1;
     float* const s_bias = (float*)(smem + 4 * TL::BYTES);
-    float* const s_sum = s_bias + width;                                   // [8][width]
+    float* const s_sum = s_bias + width;                                   // [4][width]
     const int hk = blockIdx.x % a.Hk, g = blockIdx.x / a.Hk % (a.H / a.Hk), head = hk * (a.H / a.Hk) + g;
     const int slot = a.slots - 1 - (int)(blockIdx.x / a.H);
     const bool want_table = BIAS && a.dtable_part;
@@ -464,9 +469,9 @@ __global__ __launch_bounds__(256, 2) void pa_bwd_dq_kernel(const PaArgs a) {
     if (BIAS) {
         pa_bias_fill(a, head, s_bias);
         if (want_table)
-            for (int i = threadIdx.x; i < 8 * width; i += 256) s_sum[i] = 0.f;
+            for (int i = threadIdx.x; i < 4 * width; i += 256) s_sum[i] = 0.f;
     }
-    float* const my_sum = s_sum + (threadIdx.x >> 5) * width;
+    float* const my_sum = s_sum + wave * width, *const s_tile = s_sum + 4 * width + wave * (32 * 17);   // the tile: [query][key], 17 apart
     float before = 0.f, after = 0.f, pbefore = 0.f, pafter = 0.f;          // ds and p at distances <= -far, >= far
     float all = 0.f;                                                       // every ds of the row
 
@@ -521,11 +526,14 @@ __global__ __launch_bounds__(256, 2) void pa_bwd_dq_kernel(const PaArgs a) {
     auto scores = [&](const char* lk, const char* lv, int sub, int k0, float (&p)[16], f32x16& dp) {
         f32x16 sc = pa_zero();
         dp = pa_zero();
+        __builtin_amdgcn_s_setprio(1);
 #pragma unroll
         for (int kc = 0; kc < KC; ++kc) {
             sc = pa_mfma(pa_row_frag<v8, DHP>(lk + sub * 32 * TL::RB, rp, kc), bq[kc], sc);
             dp = pa_mfma(pa_row_frag<v8, DHP>(lv + sub * 32 * TL::RB, rp, kc), bdo[kc], dp);
         }
+        pa_order<2 * KC, 1, 4>();
+        __builtin_amdgcn_s_setprio(0);
         const int dist0 = k0 + h * 4 - (qi + off), lo = k0 - (w0 + 31 + off), hi = k0 + 31 - (w0 + off);
         if (!BIAS || hi <= -a.far || lo >= a.far) {
             const float b = BIAS ? s_bias[hi <= -a.far ? 0 : 2 * a.far] - lse : -lse;
@@ -593,34 +601,45 @@ __global__ __launch_bounds__(256, 2) void pa_bwd_dq_kernel(const PaArgs a) {
                 }
                 all += sum;
                 if (want_table) {
-                    const int dist0 = k0 + h * 4 - (qi + off), lo = k0 - (w0 + 31 + off), hi = k0 + 31 - (w0 + off);
+                    const int lo = k0 - (w0 + 31 + off), hi = k0 + 31 - (w0 + off);
                     if (hi <= -a.far || lo >= a.far) {
                         float ps = 0.f;
 #pragma unroll
                         for (int i = 0; i < 16; ++i) ps += p[i];
                         if (lo >= a.far) { after += sum; pafter += ps; }
                         else { before += sum; pbefore += ps; }
-                    } else if (lo > -a.far && hi < a.far) {
-                        float* const at = my_sum + dist0 + a.far;
-#pragma unroll
-                        for (int i = 0; i < 16; ++i) __hip_atomic_fetch_add(at + (i >> 2) * 8 + (i & 3), ds[i], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
                     } else {
 #pragma unroll
-                        for (int i = 0; i < 16; ++i) {
-                            const int d = dist0 + (i >> 2) * 8 + (i & 3);
-                            if (d <= -a.far) { before += ds[i]; pbefore += p[i]; }
-                            else if (d >= a.far) { after += ds[i]; pafter += p[i]; }
-                            else __hip_atomic_fetch_add(my_sum + d + a.far, ds[i], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
+                        for (int half = 0; half < 2; ++half) {
+                            pa_wave_order();
+#pragma unroll
+                            for (int i = 0; i < 8; ++i) s_tile[col * 17 + (i >> 2) * 8 + h * 4 + (i & 3)] = ds[half * 8 + i];
+                            pa_wave_order();
+                            // lane's diagonal: key - query = lane - 31; what a lane reads off the tile's ends is dropped
+                            const float* const at = s_tile + (31 - lane) * 17;
+                            float x = 0.f;
+#pragma unroll
+                            for (int kk = 0; kk < 16; ++kk) {
+                                const float e = at[kk * 18];
+                                x += kk <= lane && kk >= lane - 31 ? e : 0.f;
+                            }
+                            const int d = k0 + half * 16 - (w0 + off) + lane - 31;
+                            if (d <= -a.far) before += x;
+                            else if (d >= a.far) after += x;
+                            else if (lane < 47) my_sum[d + a.far] += x;
                         }
                     }
                 }
                 // ds is rounded to the type of k for the product (see p in the forward pass)
+                __builtin_amdgcn_s_setprio(1);
 #pragma unroll
                 for (int c = 0; c < 2; ++c) {
                     const v8 r = pa_pack<T>(ds + 8 * c);
 #pragma unroll
                     for (int mt = 0; mt < MT; ++mt) acc[mt] = pa_mfma(pa_col_frag<v8, DHP>(lk, cp, sub * 32 + 16 * c, mt), r, acc[mt]);
                 }
+                pa_order<2 * MT, 2, 3>();
+                __builtin_amdgcn_s_setprio(0);
             }
         }
     }
@@ -636,20 +655,23 @@ __global__ __launch_bounds__(256, 2) void pa_bwd_dq_kernel(const PaArgs a) {
     for (int i = threadIdx.x; i < width; i += 256) {
         float x = 0.f;
 #pragma unroll
-        for (int k = 0; k < 8; ++k) x += s_sum[k * width + i];
+        for (int k = 0; k < 4; ++k) x += s_sum[k * width + i];
         if (i == 0) x += (s_bias[0] + s_bias[2]) + (s_bias[4] + s_bias[6]);
         if (i == 2 * a.far) x += (s_bias[1] + s_bias[3]) + (s_bias[5] + s_bias[7]);
-        s_sum[i] = x;                                  // (only this thread reads or writes column i)
+        int k = a.bucket_of[i];
+        k = k < 0 ? 0 : k >= a.buckets ? a.buckets - 1 : k;
+        s_sum[i] = x;                                  // (only this thread reads or writes column i of the four)
+        s_sum[width + i] = __int_as_float(k);
     }
     __syncthreads();
-    for (int b = threadIdx.x; b < a.buckets; b += 256) {
+    // eight lanes take a bucket, each every eighth distance
+    for (int b0 = 0; b0 < a.buckets; b0 += 32) {
+        const int b = b0 + (threadIdx.x >> 3);
         float x = 0.f;
-        for (int i = 0; i < width; ++i) {
-            int k = a.bucket_of[i];
-            k = k < 0 ? 0 : k >= a.buckets ? a.buckets - 1 : k;
-            x += k == b ? s_sum[i] : 0.f;
-        }
-        part[b] = x;
+#pragma unroll 4
+        for (int i = threadIdx.x & 7; i < width; i += 8) x += __float_as_int(s_sum[width + i]) == b ? s_sum[i] : 0.f;
+        for (int o = 1; o < 8; o <<= 1) x += __shfl_xor(x, o, 64);
+        if ((threadIdx.x & 7) == 0 && b < a.buckets) part[b] = x;
     }
 }
 
@@ -755,6 +777,7 @@ __global__ __launch_bounds__(256, 2) void pa_bwd_dkv_kernel(const PaArgs a) {
         const int q0 = first + q_tile * ROWS + sub * 32;
         if (w_rows > 0 && q0 < sq.n2 && (!a.causal || q0 + 31 + off >= w0)) {
             f32x16 sc = pa_zero(), dp = pa_zero();
+            __builtin_amdgcn_s_setprio(1);
 #pragma unroll
             for (int kc = 0; kc < KC; ++kc) sc = pa_mfma(pa_row_frag<v8, DHP>(lq + sub * 32 * TL::RB, rp, kc), bk[kc], sc);
 #pragma unroll
@@ -762,6 +785,7 @@ __global__ __launch_bounds__(256, 2) void pa_bwd_dkv_kernel(const PaArgs a) {
                 dp = pa_mfma(pa_row_frag<v8, DHP>(lp + sub * 32 * TL::RB, rp, kc), VLDS ? pa_row_frag<v8, DHP>(s_v, vp, kc) : bv[kc], dp);
             pa_order<KC, 1, 3>();
             pa_order<KC, VLDS ? 2 : 1, 2>();
+            __builtin_amdgcn_s_setprio(0);
             // (here, so that a branch ends the region in which the compiler may hold these products back and keep all their operands instead)
             if (a.causal && w0 + w_rows - 1 > q0 + off) {
                 const int firstq = ki - off - q0 - h * 4;                  // query index of a row that sees this key
@@ -791,6 +815,7 @@ __global__ __launch_bounds__(256, 2) void pa_bwd_dkv_kernel(const PaArgs a) {
 #pragma unroll
                 for (int j = 0; j < 4; ++j) p[g * 4 + j] = __builtin_amdgcn_exp2f(p[g * 4 + j] - ls[j]);
             }
+            __builtin_amdgcn_s_setprio(1);
 #pragma unroll
             for (int c = 0; c < 2; ++c) {
                 const v8 r = pa_pack<T>(p + 8 * c);
@@ -811,6 +836,7 @@ __global__ __launch_bounds__(256, 2) void pa_bwd_dkv_kernel(const PaArgs a) {
                 for (int mt = 0; mt < MT; ++mt) dk[mt] = pa_mfma(pa_col_frag<v8, DHP>(lq, cp, sub * 32 + 16 * c, mt), r, dk[mt]);
             }
             pa_order<2 * MT, 2, 3>();
+            __builtin_amdgcn_s_setprio(0);
         }
         }
         if (++q_tile == tiles) { q_tile = 0; ++q_head; }
@@ -863,6 +889,7 @@ template <typename T> __global__ __launch_bounds__(256) void pa_dkv_join_kernel(
 // ================================================================================================================================
 namespace {
 constexpr int PA_MAX_FAR = 1024;
+constexpr size_t PA_DIAGONALS = (4 * 32 * 17 + 256) * 4;      // four tiles, and what is read past the last
 
 int pa_launch(void (*kernel)(const PaArgs), dim3 grid, int threads, size_t lds, const PaArgs& a, hipStream_t st) {
     if (lds > 64 * 1024 && hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds) != hipSuccess) {
@@ -882,7 +909,7 @@ template <typename T, int DHP, bool BIAS>
 int pa_launch_bwd(PaArgs a, float* dtable, hipStream_t st) {
     const size_t width = (2 * a.far + 1) * 4;
     if (a.Tq > 0) {
-        if (const int rc = pa_launch(pa_bwd_dq_kernel<T, DHP, BIAS>, dim3((unsigned)(a.slots * a.H)), 256, 4 * PaTile<DHP>::BYTES + (BIAS ? (a.dtable_part ? 9 : 1) * width : 0), a, st)) return rc;
+        if (const int rc = pa_launch(pa_bwd_dq_kernel<T, DHP, BIAS>, dim3((unsigned)(a.slots * a.H)), 256, 4 * PaTile<DHP>::BYTES + (BIAS ? (a.dtable_part ? 5 * width + PA_DIAGONALS : width) : 0), a, st)) return rc;
     }
     if (a.dtable_part)
         hipLaunchKernelGGL(pa_dtable_kernel, dim3((unsigned)a.H), dim3(256), 0, st, a.dtable_part, a.Tq > 0 ? a.slots : 0, a.H, a.buckets, dtable);
@@ -897,13 +924,18 @@ int pa_launch_bwd(PaArgs a, float* dtable, hipStream_t st) {
     return ddpm_check_launch("packed_attention_backward");
 }
 
-// How many workgroups share the queries of 128 keys.  RULE
+// How many workgroups share the queries of 128 keys.  The host knows sizes, not lengths: `groups` of keys, and on average `steps` tiles of
+// queries for each.  Two workgroups fit on a CU and those of a causal launch differ in length, so that about four for each CU are wanted; but each
+// share is written and read once more in 32 bits, and begins with k, v.  Backward pass in us, one share against the rule's:
+//   336 groups of 74 steps (causal, 128 wide)  562 / 370 (3)      544 of 256 (causal, 128 wide)  1327 / 974 (2)     112 of 44 (causal, 64 wide)  163 / 72 (9)
+//   18 of 16 (64 wide)                          80 / 31 (8)       268 of 128 (64 wide)            446 / 328 (3)
+// and where it leaves one, against two:  512 of 19 (64 wide) 136 / 147,  176 of 8 (causal, 64 wide) 36 / 41,  4288 of 64 (causal, 128 wide) 1962 / 2337.
 int pa_splits(const ddpm_packed_attn_desc* d) {
-    const long long groups = (long long)(d->Tk / PA_ROWS + d->B + 2) * d->Hk, steps = (long long)d->Tq / PA_TILE / (d->B > 0 ? d->B : 1) * (d->H / d->Hk);
-    long long z = 512 / groups;
-    z = z < steps / 4 ? z : steps / 4;
-    if (const char* e = getenv("PAZ")) z = atoi(e);
-    return z < 1 ? 1 : z > 16 ? 16 : (int)z;
+    const long long groups = (long long)(d->Tk / PA_ROWS + d->B + 2) * d->Hk, steps = (long long)d->Tq / PA_TILE * (d->H / d->Hk) / (d->B > 0 ? d->B : 1);
+    const long long most = steps / (groups >= 128 ? 16 : 2);               // (half of the card idle: even short shares pay)
+    long long z = 1100 / groups;
+    z = z < most ? z : most;
+    return z < 1 ? 1 : z > 12 ? 12 : (int)z;
 }
 
 template <typename F> int pa_dispatch(const ddpm_packed_attn_desc* d, F&& f) {
