@@ -4,7 +4,8 @@
 //   dw = sum over rows of dy * xhat, db = sum over rows of dy
 // Both passes move every element once (x -> y; x, dy -> dx) and are bound by HBM: a row lives in registers between its loads and
 // its store, and w, b and the column sums of dw, db live in registers across the rows that a workgroup works through, so that
-// neither the parameters nor a second sweep over x and dy cost bandwidth.  The next row's loads are issued before the current
+// neither the parameters nor a second sweep over x and dy cost bandwidth (16384 x 1024 bf16: 15 us forward, 28 backward with the sums;
+// 14 and 21 at the rate of a large copy).  The next row's loads are issued before the current
 // row's reduction.  Rows of up to 1024 elements belong to a group of 4 ... 64 lanes of one wave (reduction by lane exchanges
 // only), longer ones to a workgroup of 256 or 512 threads (one barrier per row).
 //   Statistics: mean first, then squared deviations from it, both from the registers, in fp32: no difference of large sums.  Across
@@ -25,6 +26,28 @@ template <typename T, int V> __device__ __forceinline__ float vec_get(const type
 template <typename T, int V> __device__ __forceinline__ void vec_set(typename VecOf<T, V>::type& v, int j, float f) {
     if constexpr (V == 1) v = (T)f;
     else v[j] = (T)f;
+}
+
+// N consecutive floats at any multiple of 4 bytes
+template <int N> __device__ __forceinline__ void ln_get(float* f, const float* p) {
+    typedef float vec __attribute__((ext_vector_type(4), aligned(4)));
+    if constexpr (N % 4 == 0) {
+#pragma unroll
+        for (int j = 0; j < N; j += 4) {
+            const vec v = *(const vec*)(p + j);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) f[j + i] = v[i];
+        }
+    } else
+        f[0] = *p;
+}
+template <int N> __device__ __forceinline__ void ln_put(float* p, const float* f) {
+    typedef float vec __attribute__((ext_vector_type(4), aligned(4)));
+    if constexpr (N % 4 == 0) {
+#pragma unroll
+        for (int j = 0; j < N; j += 4) *(vec*)(p + j) = vec{f[j], f[j + 1], f[j + 2], f[j + 3]};
+    } else
+        *p = f[0];
 }
 
 struct LnArgs {
@@ -55,14 +78,16 @@ __global__ __launch_bounds__(BLOCK ? BLOCK : 256) void ln_fwd_kernel(const LnArg
     float w[NV * V], b[NV * V];
     int count = 0;
 #pragma unroll
-    for (int v = 0; v < NV; ++v)
+    for (int v = 0; v < NV; ++v) {
+        const int c = (v * tpr + t) * V;
 #pragma unroll
-        for (int j = 0; j < V; ++j) {
-            const int c = (v * tpr + t) * V + j;
-            w[v * V + j] = a.w && c < a.C ? a.w[c] : 1.f;
-            b[v * V + j] = a.b && c < a.C ? a.b[c] : 0.f;
-            count += c < a.C;
+        for (int j = 0; j < V; ++j) { w[v * V + j] = 1.f; b[v * V + j] = 0.f; }
+        if (c < a.C) {
+            if (a.w) ln_get<V>(w + v * V, a.w + c);
+            if (a.b) ln_get<V>(b + v * V, a.b + c);
+            count += V;
         }
+    }
     // the wave's share of a row: its size (LDS: of every wave) and reciprocal
     __shared__ float s_n[WAVES];
     const float n_w = BLOCK ? group_sum((float)count, 64) : 0.f, inv_n = n_w > 0.f ? 1.f / n_w : 0.f;
@@ -143,10 +168,11 @@ __global__ __launch_bounds__(BLOCK ? BLOCK : 256) void ln_bwd_kernel(const LnArg
     T* const dx = (T*)a.dx;
     float w[E], dw[E], db[E];
 #pragma unroll
-    for (int i = 0; i < E; ++i) {
-        const int c = (i / V * tpr + t) * V + i % V;
-        w[i] = a.w && c < a.C ? a.w[c] : 1.f;
-        dw[i] = db[i] = 0.f;
+    for (int v = 0; v < NV; ++v) {
+        const int c = (v * tpr + t) * V;
+#pragma unroll
+        for (int j = 0; j < V; ++j) { w[v * V + j] = 1.f; dw[v * V + j] = db[v * V + j] = 0.f; }
+        if (a.w && c < a.C) ln_get<V>(w + v * V, a.w + c);
     }
     vec nx[NV], nd[NV];
     float2 nst = make_float2(0.f, 0.f);
@@ -207,18 +233,26 @@ __global__ __launch_bounds__(BLOCK ? BLOCK : 256) void ln_bwd_kernel(const LnArg
     float* const part = a.part + (long long)blockIdx.x * 2 * a.C;
     if constexpr (BLOCK != 0) {
 #pragma unroll
-        for (int i = 0; i < E; ++i) {
-            const int c = (i / V * tpr + t) * V + i % V;
-            if (c < a.C) { part[c] = dw[i]; part[a.C + c] = db[i]; }
+        for (int v = 0; v < NV; ++v) {
+            const int c = (v * tpr + t) * V;
+            if (c < a.C) {
+                ln_put<V>(part + c, dw + v * V);
+                ln_put<V>(part + a.C + c, db + v * V);
+            }
         }
     } else {
         // lane groups of the wave, then the four waves through LDS, each in a fixed order
         float* const mine = s_col + (tid >> 6) * 2 * a.C;
 #pragma unroll
-        for (int i = 0; i < E; ++i) {
+        for (int i = 0; i < E; ++i)
             for (int o = tpr; o < 64; o <<= 1) { dw[i] += __shfl_xor(dw[i], o, 64); db[i] += __shfl_xor(db[i], o, 64); }
-            const int c = (i / V * tpr + t) * V + i % V;
-            if ((tid & 63) < tpr && c < a.C) { mine[c] = dw[i]; mine[a.C + c] = db[i]; }
+#pragma unroll
+        for (int v = 0; v < NV; ++v) {
+            const int c = (v * tpr + t) * V;
+            if ((tid & 63) < tpr && c < a.C) {
+                ln_put<V>(mine + c, dw + v * V);
+                ln_put<V>(mine + a.C + c, db + v * V);
+            }
         }
         __syncthreads();
         for (int i = tid; i < 2 * a.C; i += 256) part[i] = (s_col[i] + s_col[2 * a.C + i]) + (s_col[4 * a.C + i] + s_col[6 * a.C + i]);
@@ -265,9 +299,12 @@ bool ln_plan(long long rows, int C, bool aligned, int size, bool fwd, LnPlan& p)
     p.nv = 1;
     while (p.nv < need) p.nv *= 2;
     const long long groups = p.block ? rows : (rows + 256 / p.tpr - 1) / (256 / p.tpr);
-    // forward: as many waves as the card holds at once; backward: half of them (its registers allow no more), which also
-    // bounds the workspace of partial sums
-    const long long cap = (p.block == 512 ? 1024 : 2048) / (fwd ? 1 : 2);
+    // Workgroups per CU: enough loads in flight for HBM, but each begins with w, b (and ends with the column sums), which the rows it works
+    // through have to pay for.  us at 65536 x 4096 bf16: forward 218 / 200 / 182 with 6 / 3 / 2 a CU, but 59 / 49 / 60 at 20000 x 3000; a wave to
+    // a row, 65536 x 512: 37 / 28 / 28 with 3 / 6 / 8.  Backward, 65536 x 4096: 337 / 293 with 4 / 2; 8192 x 8192: 86 / 80 with 2 / 1; a wave to a
+    // row of 16384 x 1024: 34 / 28 with 4 / 2, of 65536 x 512: 45 / 58.
+    const int per_cu = fwd ? (p.block == 0 ? 6 : p.block == 256 ? 3 : 2) : p.block == 512 ? 1 : p.block == 256 || p.nv * V == 16 ? 2 : 4;
+    const long long cap = 256 * per_cu;
     p.grid = (int)(groups < cap ? groups : cap);
     return p.nv <= most;
 }

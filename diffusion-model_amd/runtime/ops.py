@@ -562,13 +562,16 @@ def packed_attention_backward(q: Tensor, k: Tensor, v: Tensor, o: Tensor, lse: T
     dq, dk, dv = (torch.empty(t.shape, device=t.device, dtype=t.dtype) for t in (q, k, v)) if grads is None else grads
     assert dout.shape == q.shape and dout.dtype == q.dtype and lse.shape == (q.shape[1], q.shape[0]) and lse.is_contiguous()
     assert all(t.stride(2) == 1 for t in (q, k, v, o, dout, dq, dk, dv)) and (not want_dtable or o32 is not None)
-    dsum = torch.empty_like(lse)
     dtable = torch.empty_like(table) if want_dtable else None
-    part = torch.empty(hip.lib().ddpm_packed_attn_slots(d.Tq, d.B) * d.H * d.buckets, device=q.device, dtype=torch.float32) if want_dtable else None
-    d.lse, d.dsum, d.o32, d.dtable, d.dtable_part = lse.data_ptr(), dsum.data_ptr(), hip.ptr(o32), hip.ptr(dtable), hip.ptr(part)
-    floats = hip.lib().ddpm_packed_attn_dkv_floats(C.byref(d))
-    split = torch.empty(floats, device=q.device, dtype=torch.float32) if floats else None
-    d.dkv_part = hip.ptr(split)
+    # one allocation for the workspaces (fp32): D of every row, partial sums of the table's gradient, shares of dk and dv
+    rows, part = lse.numel(), hip.lib().ddpm_packed_attn_slots(d.Tq, d.B) * d.H * d.buckets if want_dtable else 0
+    part = (part + 3) // 4 * 4
+    split = hip.lib().ddpm_packed_attn_dkv_floats(C.byref(d))
+    space = torch.empty((rows + 3) // 4 * 4 + part + split, device=q.device, dtype=torch.float32)
+    work = space.data_ptr
+    d.lse, d.dsum, d.o32, d.dtable = lse.data_ptr(), work(), hip.ptr(o32), hip.ptr(dtable)
+    d.dtable_part = work() + (rows + 3) // 4 * 16 if part else None
+    d.dkv_part = work() + (rows + 3) // 4 * 16 + 4 * part if split else None
     d.o, d.o_row, d.o_head, d.dout, d.dout_row, d.dout_head = o.data_ptr(), o.stride(0), o.stride(1), dout.data_ptr(), dout.stride(0), dout.stride(1)
     d.dq, d.dq_row, d.dq_head, d.dk, d.dk_row, d.dk_head = dq.data_ptr(), dq.stride(0), dq.stride(1), dk.data_ptr(), dk.stride(0), dk.stride(1)
     d.dv, d.dv_row, d.dv_head = dv.data_ptr(), dv.stride(0), dv.stride(1)
