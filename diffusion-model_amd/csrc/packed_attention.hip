@@ -16,9 +16,8 @@
 // operand of that product is read transposed from the same LDS tile (ds_read_b64_tr_b16).  Rows of a tile are stored with their 16-byte
 // pieces exchanged by a row-dependent xor, so that the lanes of either kind of read fall on different banks.
 //
-// Sequences.  The launch has one slot for every 128 rows plus one per sequence: floor(begin / 128) + index never collides and needs no
-// host knowledge of the lengths.  A workgroup finds its sequence from the boundaries by one load and a ballot.  Rows outside of all
-// sequences are two more sequences without keys: their results are zeros where the caller wants that, and they are not touched otherwise.
+// Sequences.  The launch has one slot for every 128 rows plus one per sequence, which is enough whatever the lengths are; the host does not know
+// them.  A workgroup finds its sequence from the boundaries, a lane to each.  Rows outside of all sequences are two more sequences without keys: their results are zeros where the caller wants that, and they are not touched otherwise.
 // Boundaries are clamped to the tensors, so that no contents of that array reach outside of them.
 #include <type_traits>
 #include "common.h"
@@ -98,7 +97,6 @@ struct PaSeq {
     int begin, n;            // rows of the side that the launch's slots run over
     int begin2, n2;          // rows of the other side
     int row0;                // first of this workgroup's rows, counted from begin
-    bool real;
 };
 
 // s = 0: the rows in front of the first sequence, s = B + 1: those behind the last
@@ -109,33 +107,57 @@ __device__ __forceinline__ int pa_bound(const int* ends, int s, int B, int T) {
     return e < 0 ? 0 : e > T ? T : e;
 }
 
-__device__ __forceinline__ bool pa_find(const int* ends, int T, const int* ends2, int T2, int B, int slot, PaSeq& r) {
+// The workgroup's rows: `rank` counts the tiles of 128 rows of all sequences, those with the most of the other side's rows first, so that the
+// longest workgroups of a causal launch begin first and short ones fill the end: by the tile's index within its sequence, from the
+// highest (queries: a later one sees more keys), or from the sequence's end (keys: an earlier one is seen by more queries).  A lane holds a
+// sequence's number of tiles; the level that the rank falls into is found by bisection.  More sequences than lanes: by slots, in order.
+template <bool KEYS>
+__device__ __forceinline__ bool pa_find(const int* ends, int T, const int* ends2, int T2, int B, int zero_rest, int rank, int slots, PaSeq& r) {
     const int lane = threadIdx.x & 63;
-    int before = 0;
-    for (int s0 = 0; s0 < B + 2; s0 += 64) {
-        const int s = s0 + lane;
-        const bool in = s < B + 2 && pa_bound(ends, s, B, T) / PA_ROWS + s <= slot;
-        before += __popcll(__ballot(in));
+    int s;
+    if (B + 2 <= 64) {
+        const int begin = lane < B + 2 ? pa_bound(ends, lane, B, T) : T, end = lane < B + 2 ? pa_bound(ends, lane + 1, B, T) : T;
+        const bool real = lane >= 1 && lane <= B;
+        const int tiles = end > begin && (real || zero_rest) ? (end - begin + PA_ROWS - 1) / PA_ROWS : 0;
+        auto beyond = [&](int level) {                                     // tiles at this level and above
+            int v = tiles > level ? tiles - level : 0;
+#pragma unroll
+            for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
+            return __builtin_amdgcn_readfirstlane(v);
+        };
+        if (beyond(0) <= rank) return false;
+        int level = 0, above = -1;
+        for (int bit = 1 << (31 - __builtin_clz(T / PA_ROWS + 1)); bit > 0; bit >>= 1) {
+            const int n = beyond(level + bit);
+            if (n > rank) level += bit;
+            else above = n;                                                // (of the lowest level tried that is too high: level + 1 in the end)
+        }
+        const unsigned long long at = __ballot(tiles > level);
+        const int before = __popcll(at & ((1ull << lane) - 1));
+        s = __ffsll(__ballot(tiles > level && before == rank - above)) - 1;
+        r.begin = __builtin_amdgcn_readlane(begin, s);
+        r.n = __builtin_amdgcn_readlane(end, s) - r.begin;
+        r.row0 = (KEYS ? __builtin_amdgcn_readlane(tiles, s) - 1 - level : level) * PA_ROWS;
+    } else {
+        const int slot = KEYS ? rank : slots - 1 - rank;
+        int before = 0;
+        for (int s0 = 0; s0 < B + 2; s0 += 64)
+            before += __popcll(__ballot(s0 + lane < B + 2 && pa_bound(ends, s0 + lane, B, T) / PA_ROWS + s0 + lane <= slot));
+        s = __builtin_amdgcn_readfirstlane(before) - 1;
+        if (s < 0) return false;
+        r.begin = __builtin_amdgcn_readfirstlane(pa_bound(ends, s, B, T));
+        r.n = __builtin_amdgcn_readfirstlane(pa_bound(ends, s + 1, B, T)) - r.begin;
+        r.row0 = (slot - (r.begin / PA_ROWS + s)) * PA_ROWS;
+        if (r.row0 < 0 || r.row0 >= r.n) return false;
     }
-    const int s = __builtin_amdgcn_readfirstlane(before) - 1;
-    if (s < 0) return false;
-    r.begin = pa_bound(ends, s, B, T);
-    const int end = pa_bound(ends, s + 1, B, T);
-    r.n = end > r.begin ? end - r.begin : 0;
-    r.row0 = (slot - (r.begin / PA_ROWS + s)) * PA_ROWS;
-    r.real = s >= 1 && s <= B;
+    const bool real = s >= 1 && s <= B;
     r.begin2 = r.n2 = 0;
-    if (r.real) {
-        r.begin2 = pa_bound(ends2, s, B, T2);
-        const int end2 = pa_bound(ends2, s + 1, B, T2);
+    if (real) {
+        r.begin2 = __builtin_amdgcn_readfirstlane(pa_bound(ends2, s, B, T2));
+        const int end2 = __builtin_amdgcn_readfirstlane(pa_bound(ends2, s + 1, B, T2));
         r.n2 = end2 > r.begin2 ? end2 - r.begin2 : 0;
     }
-    r.begin = __builtin_amdgcn_readfirstlane(r.begin);
-    r.n = __builtin_amdgcn_readfirstlane(r.n);
-    r.begin2 = __builtin_amdgcn_readfirstlane(r.begin2);
-    r.n2 = __builtin_amdgcn_readfirstlane(r.n2);
-    r.row0 = __builtin_amdgcn_readfirstlane(r.row0);
-    return r.row0 >= 0 && r.row0 < r.n;
+    return real || zero_rest;
 }
 
 // ---- tiles -------------------------------------------------------------------------------------------------------------------
@@ -281,10 +303,8 @@ __global__ __launch_bounds__(256, 2) void pa_fwd_kernel(const PaArgs a) {
     float* const s_bias = (float*)(smem + 4 * TL::BYTES);
     // heads that share k, v differ by Hk in their index: with workgroups dealt to the eight XCDs in turn, they meet in one L2
     const int hk = blockIdx.x % a.Hk, g = blockIdx.x / a.Hk % (a.H / a.Hk), head = hk * (a.H / a.Hk) + g;
-    const int slot = a.slots - 1 - (int)(blockIdx.x / a.H);                // (ends of causal sequences, the longest rows, first)
     PaSeq sq;
-    if (!pa_find(a.ends_q, a.Tq, a.ends_k, a.Tk, a.B, slot, sq)) return;
-    if (!sq.real && !a.zero_rest) return;
+    if (!pa_find<false>(a.ends_q, a.Tq, a.ends_k, a.Tk, a.B, a.zero_rest, (int)(blockIdx.x / a.H), a.slots, sq)) return;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), col = lane & 31, h = lane >> 5;
     const int w0 = sq.row0 + wave * 32, qi = w0 + col;                     // the wave's first row, the lane's row
     const bool qv = qi < sq.n;
@@ -452,11 +472,11 @@ __global__ __launch_bounds__(256, 2) void pa_bwd_dq_kernel(const PaArgs a) {
     float* const s_bias = (float*)(smem + 4 * TL::BYTES);
     float* const s_sum = s_bias + width;                                   // [4][width]
     const int hk = blockIdx.x % a.Hk, g = blockIdx.x / a.Hk % (a.H / a.Hk), head = hk * (a.H / a.Hk) + g;
-    const int slot = a.slots - 1 - (int)(blockIdx.x / a.H);
+    const int rank = (int)(blockIdx.x / a.H);
     const bool want_table = BIAS && a.dtable_part;
-    float* const part = want_table ? a.dtable_part + ((long long)slot * a.H + head) * a.buckets : nullptr;
+    float* const part = want_table ? a.dtable_part + ((long long)rank * a.H + head) * a.buckets : nullptr;
     PaSeq sq;
-    if (!pa_find(a.ends_q, a.Tq, a.ends_k, a.Tk, a.B, slot, sq) || (!sq.real && !a.zero_rest)) {
+    if (!pa_find<false>(a.ends_q, a.Tq, a.ends_k, a.Tk, a.B, a.zero_rest, rank, a.slots, sq)) {
         if (want_table)
             for (int i = threadIdx.x; i < a.buckets; i += 256) part[i] = 0.f;
         return;
@@ -704,10 +724,9 @@ __global__ __launch_bounds__(256, 2) void pa_bwd_dkv_kernel(const PaArgs a) {
     float* const s_row = (float*)(smem + 4 * TL::BYTES);                   // [2][2][ROWS]
     float* const s_bias = s_row + 4 * ROWS;
     const int hk = blockIdx.x % a.Hk, group = a.H / a.Hk;
-    const int slot = (int)(blockIdx.x / (a.Hk * a.splits)), split = __builtin_amdgcn_readfirstlane((int)(blockIdx.x / a.Hk % a.splits));   // (starts of causal sequences, the most queries, first)
+    const int split = __builtin_amdgcn_readfirstlane((int)(blockIdx.x / a.Hk % a.splits));
     PaSeq sq;                                                              // begin, n: keys; begin2, n2: queries
-    if (!pa_find(a.ends_k, a.Tk, a.ends_q, a.Tq, a.B, slot, sq)) return;
-    if (!sq.real && !a.zero_rest) return;
+    if (!pa_find<true>(a.ends_k, a.Tk, a.ends_q, a.Tq, a.B, a.zero_rest, (int)(blockIdx.x / (a.Hk * a.splits)), a.slots, sq)) return;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), col = lane & 31, h = lane >> 5;
     const int w0 = sq.row0 + wave * 32, ki = w0 + col;
     const bool kv = ki < sq.n;
