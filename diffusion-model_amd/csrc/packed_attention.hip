@@ -294,7 +294,8 @@ __device__ __forceinline__ int pa_clamp(int d, int far) { return d < -far ? -far
 // ================================================================================================================================
 // forward
 // ================================================================================================================================
-template <typename T, int DHP, bool BIAS>
+// TWO: with a bias whose gradient will be wanted, from p in two parts
+template <typename T, int DHP, bool BIAS, bool TWO>
 __global__ __launch_bounds__(256, 2) void pa_fwd_kernel(const PaArgs a) {
     typedef typename PaTypes<T>::v8 v8;
     typedef PaTile<DHP> TL;
@@ -332,8 +333,12 @@ __global__ __launch_bounds__(256, 2) void pa_fwd_kernel(const PaArgs a) {
         pa_load<DHP, PA_TILE>(to + TL::BYTES, vb, a.v.row, t * PA_TILE, sq.n2, a.dh, vo);
     };
     if (tiles > 0) fetch(0);
-    const unsigned rp = pa_row_place<DHP>(col, h), cp = pa_col_place<DHP>();
+    unsigned rp = pa_row_place<DHP>(col, h), cp = pa_col_place<DHP>();
     for (int t = 0; t < tiles; ++t) {
+        if (BIAS) {
+            pa_opaque<DHP>(rp);
+            pa_opaque<DHP>(cp);
+        }
         const char* const lk = smem + (t & 1) * 2 * TL::BYTES;
         const char* const lv = lk + TL::BYTES;
         const int k0 = t * PA_TILE;
@@ -369,7 +374,7 @@ __global__ __launch_bounds__(256, 2) void pa_fwd_kernel(const PaArgs a) {
                 }
             } else {
 #pragma unroll
-                for (int i = 0; i < 32; ++i) s[i] = sc[i >> 4][i & 15] * a.scale2;
+                for (int i = 0; i < 32; ++i) s[i] = sc[i >> 4][i & 15];    // (scaled where the maximum is subtracted, in one instruction)
             }
             if (k0 + PA_TILE > sq.n2 || (a.causal && k0 + PA_TILE - 1 > w0 + off)) {
                 // key index - k0 of score i is (i >> 2) * 8 + h * 4 + (i & 3): beyond `last` it is not seen
@@ -377,10 +382,11 @@ __global__ __launch_bounds__(256, 2) void pa_fwd_kernel(const PaArgs a) {
 #pragma unroll
                 for (int i = 0; i < 32; ++i) s[i] = (i >> 2) * 8 + (i & 3) <= last ? s[i] : -INFINITY;
             }
+            const float unit = BIAS ? 1.f : a.scale2;                      // (positive: the maximum may be taken before)
             float mx = s[0];
 #pragma unroll
             for (int i = 1; i < 32; ++i) mx = fmaxf(mx, s[i]);
-            mx = pa_half_max(mx);
+            mx = pa_half_max(mx) * unit;
             // The maximum moves only when a row's grows by more than 2^8: until then the old one keeps every term below 2^8, which
             // costs no precision, and the accumulators need no rescaling.
             if (__any(mx > m + 8.f)) {
@@ -397,33 +403,29 @@ __global__ __launch_bounds__(256, 2) void pa_fwd_kernel(const PaArgs a) {
             float sum = 0.f;
 #pragma unroll
             for (int i = 0; i < 32; ++i) {
-                s[i] = __builtin_amdgcn_exp2f(s[i] - ref);
+                s[i] = __builtin_amdgcn_exp2f(s[i] * unit - ref);
                 sum += s[i];
             }
             l += sum;                                                      // (this half-wave's keys; joined at the end)
             // p is rounded to the type of v for the product (relative 2^-8 of each term in bf16, of either sign); the sum above is not.
             // Where the output feeds the bias's gradient, whose terms cancel, what that rounding leaves is multiplied as well.
             __builtin_amdgcn_s_setprio(1);
-            auto pv = [&](auto two) {
 #pragma unroll
-                for (int c = 0; c < 4; ++c) {
-                    const v8 p = pa_pack<T>(s + 8 * c);
-                    v8 rest;
-                    if constexpr (decltype(two)::value) {
+            for (int c = 0; c < 4; ++c) {
+                const v8 p = pa_pack<T>(s + 8 * c);
+                v8 rest;
+                if constexpr (TWO) {
 #pragma unroll
-                        for (int j = 0; j < 8; ++j) rest[j] = (T)(s[8 * c + j] - (float)p[j]);
-                    }
-#pragma unroll
-                    for (int mt = 0; mt < MT; ++mt) {
-                        const v8 f = pa_col_frag<v8, DHP>(lv, cp, 16 * c, mt);
-                        acc[mt] = pa_mfma(f, p, acc[mt]);
-                        if constexpr (decltype(two)::value) acc[mt] = pa_mfma(f, rest, acc[mt]);
-                    }
+                    for (int j = 0; j < 8; ++j) rest[j] = (T)(s[8 * c + j] - (float)p[j]);
                 }
-            };
-            if (BIAS && a.o32) pv(std::true_type());
-            else pv(std::false_type());
-            pa_order<4 * MT, 2, 3>();
+#pragma unroll
+                for (int mt = 0; mt < MT; ++mt) {
+                    const v8 f = pa_col_frag<v8, DHP>(lv, cp, 16 * c, mt);
+                    acc[mt] = pa_mfma(f, p, acc[mt]);
+                    if constexpr (TWO) acc[mt] = pa_mfma(f, rest, acc[mt]);
+                }
+            }
+            if (!TWO) pa_order<4 * MT, 2, 3>();
             __builtin_amdgcn_s_setprio(0);
         }
     }
@@ -921,7 +923,7 @@ int pa_launch(void (*kernel)(const PaArgs), dim3 grid, int threads, size_t lds, 
 
 template <typename T, int DHP, bool BIAS>
 int pa_launch_fwd(const PaArgs& a, hipStream_t st) {
-    return pa_launch(pa_fwd_kernel<T, DHP, BIAS>, dim3((unsigned)(a.slots * a.H)), 256, 4 * PaTile<DHP>::BYTES + (BIAS ? (2 * a.far + 1) * 4 : 0), a, st);
+    return pa_launch(BIAS && a.o32 ? pa_fwd_kernel<T, DHP, BIAS, BIAS> : pa_fwd_kernel<T, DHP, BIAS, false>, dim3((unsigned)(a.slots * a.H)), 256, 4 * PaTile<DHP>::BYTES + (BIAS ? (2 * a.far + 1) * 4 : 0), a, st);
 }
 
 template <typename T, int DHP, bool BIAS>
