@@ -82,7 +82,8 @@ class LayerNorm(nn.Module):
 # ---- attention over packed sequences ----------------------------------------------------------------------------------------
 def _heads(t: Tensor) -> Tensor:
     """t [tokens, heads, width] as the kernels read it: contiguous heads, 16-byte aligned, no two on each other; copied where it is not"""
-    fits = t.stride(2) == 1 and t.data_ptr() % 16 == 0 and all(t.shape[i] <= 1 or (t.stride(i) >= t.shape[2] and t.stride(i) % 8 == 0) for i in (0, 1))
+    (rows, heads, width), (row, head, one) = t.shape, t.stride()
+    fits = one == 1 and t.data_ptr() % 16 == 0 and (rows <= 1 or (row >= width and row % 8 == 0)) and (heads <= 1 or (head >= width and head % 8 == 0))
     return t if fits else t.clone(memory_format=torch.contiguous_format)
 
 

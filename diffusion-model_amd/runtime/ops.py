@@ -2,6 +2,7 @@
 from __future__ import annotations
 
 import ctypes as C
+import operator
 import os
 from typing import Optional
 
@@ -516,15 +517,15 @@ def _packed_desc(q: Tensor, k: Tensor, v: Tensor, ends_q: Tensor, ends_k: Option
     if q.dtype not in (BF16, torch.float16) or k.dtype != q.dtype or v.dtype != q.dtype:
         raise ValueError(f"packed_attention: q, k, v of types {q.dtype}, {k.dtype}, {v.dtype} (all bfloat16 or all float16)")
     ek = ends_q if ends_k is None else ends_k
-    for e in (ends_q, ek):
+    for e in (ends_q,) if ends_k is None else (ends_q, ek):
         if e.dtype != torch.int32 or e.dim() != 1 or e.numel() < 1 or not e.is_contiguous() or e.numel() != ends_q.numel() or e.device != q.device:
             raise ValueError("packed_attention: the sequences' boundaries are contiguous int32 tensors of (sequences + 1) beside q")
     if (table is None) != (bucket_of is None):
         raise ValueError("packed_attention: the position bias needs both its table and the buckets of the distances")
-    d = hip.PackedAttnDesc(q=q.data_ptr(), k=k.data_ptr(), v=v.data_ptr(), q_row=q.stride(0), q_head=q.stride(1), k_row=k.stride(0), k_head=k.stride(1),
-                           v_row=v.stride(0), v_head=v.stride(1), ends_q=ends_q.data_ptr(), ends_k=ek.data_ptr(), Tq=q.shape[0], Tk=k.shape[0],
-                           B=ends_q.numel() - 1, H=q.shape[1], Hk=k.shape[1], dh=q.shape[2], dtype=hip.DTYPE[q.dtype], causal=int(causal),
-                           zero_rest=int(zero_rest), scale=q.shape[2] ** -0.5 if scale is None else scale)
+    (tq, h, width), (tk, hk, _), (qr, qh, _), (kr, kh, _), (vr, vh, _) = q.shape, k.shape, q.stride(), k.stride(), v.stride()
+    d = hip.PackedAttnDesc(q=q.data_ptr(), k=k.data_ptr(), v=v.data_ptr(), q_row=qr, q_head=qh, k_row=kr, k_head=kh, v_row=vr, v_head=vh,
+                           ends_q=ends_q.data_ptr(), ends_k=ek.data_ptr(), Tq=tq, Tk=tk, B=ends_q.numel() - 1, H=h, Hk=hk, dh=width, dtype=hip.DTYPE[q.dtype],
+                           causal=int(causal), zero_rest=int(zero_rest), scale=width ** -0.5 if scale is None else scale)
     if table is not None:
         if table.dtype != torch.float32 or table.dim() != 2 or table.shape[1] != q.shape[1] or not table.is_contiguous() or table.device != q.device:
             raise ValueError(f"packed_attention: the bias table is a contiguous float32 [buckets, {q.shape[1]}] tensor beside q, got {tuple(table.shape)} {table.dtype}")
@@ -612,25 +613,26 @@ def sample_norm_backward(a: Tensor, b: Optional[Tensor], dy: Tensor, act: int, g
     return du, (da if act else du)
 
 
-def _ln_desc(x: Tensor, w: Optional[Tensor], b: Optional[Tensor], stats: Optional[Tensor], eps: float, **more) -> hip.LayerNormDesc:
-    rows, c = x.shape
+def _ln_params(x: Tensor, *params) -> None:
     if x.dtype not in hip.DTYPE:
         raise ValueError(f"layer_norm: elements of type {x.dtype} (bfloat16, float16 or float32)")
-    for t in (w, b):
-        if t is not None and (t.dtype != torch.float32 or t.shape != (c,) or not t.is_contiguous() or t.device != x.device):
-            raise ValueError(f"layer_norm: weight and bias are contiguous float32 tensors of {c} elements beside x")
-    return hip.LayerNormDesc(x=hip.ptr(x), w=hip.ptr(w), b=hip.ptr(b), stats=hip.ptr(stats), rows=rows, C=c, ldx=x.stride(0), dtype=hip.DTYPE[x.dtype],
-                             eps=eps, **more)
+    for t in params:
+        if t is not None and (t.dtype != torch.float32 or t.shape != x.shape[1:] or not t.is_contiguous() or t.device != x.device):
+            raise ValueError(f"layer_norm: weight and bias are contiguous float32 tensors of {x.shape[1]} elements beside x")
 
 
 def layer_norm_forward(x: Tensor, w: Optional[Tensor], b: Optional[Tensor], eps: float = 1e-5, *, want_stats: bool = True, out: Optional[Tensor] = None):
     """Layer norm of every row of x [rows, C] (bf16, fp16 or fp32; rows any number of elements apart, e.g. a column slice); w, b: fp32
     [C] or None.  Returns (y, stats fp32 [rows, 2] or None)."""
+    _ln_params(x, w, b)
     rows, c = x.shape
-    y = torch.empty(rows, c, device=x.device, dtype=x.dtype) if out is None else out
-    assert x.stride(1) == 1 and y.shape == x.shape and y.dtype == x.dtype and y.stride(1) == 1
+    y = x.new_empty(rows, c) if out is None else out
+    (ldx, one), (ldy, one_y) = x.stride(), y.stride()
+    assert one == 1 and one_y == 1 and y.shape == x.shape and y.dtype == x.dtype
     stats = torch.empty(rows, 2, device=x.device, dtype=torch.float32) if want_stats else None
-    d = _ln_desc(x, w, b, stats, eps, y=hip.ptr(y), ldy=y.stride(0))
+    # (fields in the order of ddpm_layer_norm_desc: by position, which halves the cost of filling one in)
+    d = hip.LayerNormDesc(x.data_ptr(), None, y.data_ptr(), None, hip.ptr(w), hip.ptr(b), hip.ptr(stats), None, None, None,
+                          rows, ldx, ldy, 0, 0, c, hip.DTYPE[x.dtype], eps)
     with hip.on_device_of(x):
         _launch("ln_fwd_kernel", lambda: (_nb(x, y, w, b, stats), 8.0 * x.numel(), f"R{rows} C{c}"),
                 lambda: hip.call("ddpm_layer_norm_forward", C.byref(d), hip.stream()))
@@ -640,24 +642,29 @@ def layer_norm_forward(x: Tensor, w: Optional[Tensor], b: Optional[Tensor], eps:
 def layer_norm_backward(x: Tensor, dy: Tensor, w: Optional[Tensor], stats: Tensor, *, want_dx: bool = True, want_dw: bool = True,
                         want_db: bool = True):
     """Gradients of layer_norm_forward: (dx like x or None, dw fp32 [C] or None, db fp32 [C] or None)."""
+    _ln_params(x, w)
     rows, c = x.shape
-    assert dy.shape == x.shape and dy.dtype == x.dtype and dy.stride(1) == 1 and x.stride(1) == 1
+    (ldx, one), (lddy, one_dy) = x.stride(), dy.stride()
+    assert dy.shape == x.shape and dy.dtype == x.dtype and one == 1 and one_dy == 1
     assert stats.shape == (rows, 2) and stats.dtype == torch.float32 and stats.is_contiguous()
-    dx = torch.empty(rows, c, device=x.device, dtype=x.dtype) if want_dx else None
-    dw = torch.empty(c, device=x.device, dtype=torch.float32) if want_dw else None
-    db = torch.empty(c, device=x.device, dtype=torch.float32) if want_db else None
-    d = _ln_desc(x, w, None, stats, 0.0, dy=hip.ptr(dy), lddy=dy.stride(0), dx=hip.ptr(dx), lddx=c, dw=hip.ptr(dw), db=hip.ptr(db))
-    part = None
+    dx = x.new_empty(rows, c) if want_dx else None
+    dw = stats.new_empty(c) if want_dw else None
+    db = stats.new_empty(c) if want_db else None
+    d = hip.LayerNormDesc(x.data_ptr(), dy.data_ptr(), None, hip.ptr(dx), hip.ptr(w), None, stats.data_ptr(), None, hip.ptr(dw), hip.ptr(db),
+                          rows, ldx, 0, lddy, c, c, hip.DTYPE[x.dtype], 0.0)
     if want_dw or want_db:
         n = hip.lib().ddpm_layer_norm_part_rows(C.byref(d))
         if n < 0:
             hip.check(n, "layer_norm_backward")
-        part = torch.empty(n, 2, c, device=x.device, dtype=torch.float32)
-        d.part = hip.ptr(part)
+        part = stats.new_empty(n, 2, c)
+        d.part = part.data_ptr()
     with hip.on_device_of(x):
         _launch("ln_bwd_kernel", lambda: (_nb(x, dy, dx, w, stats, dw, db), 12.0 * x.numel(), f"R{rows} C{c}"),
                 lambda: hip.call("ddpm_layer_norm_backward", C.byref(d), hip.stream()))
     return dx, dw, db
+
+
+_DTYPE_OF = operator.attrgetter("dtype")
 
 
 def grad_norm(grads, norm_type: float = 2.0, max_norm: Optional[float] = None) -> Tensor:
@@ -675,11 +682,10 @@ def grad_norm(grads, norm_type: float = 2.0, max_norm: Optional[float] = None) -
         raise RuntimeError("grad_norm runs on the HIP kernels only: gradients must live on an MI355X (cuda) device")
     if len(index) > 1:
         raise ValueError("grad_norm: all gradients must be on one device")
-    dev = grads[0].device
-    try:
-        size = np.fromiter((hip.DTYPE[g.dtype] for g in grads), np.uint8, count)
-    except KeyError as e:
-        raise ValueError(f"grad_norm: gradients of type {e} (bfloat16, float16 or float32)") from None
+    dev, types = grads[0].device, list(map(_DTYPE_OF, grads))
+    if not hip.DTYPE.keys() >= set(types):
+        raise ValueError(f"grad_norm: gradients of types {set(types)} (bfloat16, float16 or float32)")
+    size = np.fromiter(map(hip.DTYPE.__getitem__, types), np.uint8, count)
     if not all(map(Tensor.is_contiguous, grads)):
         for g in grads:
             if g.layout != torch.strided or not torch.ops.aten.is_non_overlapping_and_dense(g):
