@@ -107,57 +107,67 @@ __device__ __forceinline__ int pa_bound(const int* ends, int s, int B, int T) {
     return e < 0 ? 0 : e > T ? T : e;
 }
 
+// sum over the lanes up to and including this one, without a trip through LDS (data-parallel moves within rows of 16, then across)
+__device__ __forceinline__ int pa_scan(int v) {
+    v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xf, 0xf, false);        // row_shr 1, 2, 4, 8
+    v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xf, 0xf, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xf, 0xf, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xf, 0xf, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xa, 0xf, false);        // the last of rows 0 and 2 to rows 1 and 3
+    v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xc, 0xf, false);        // the last of row 1 to rows 2 and 3
+    return v;
+}
+
 // The workgroup's rows: `rank` counts the tiles of 128 rows of all sequences, those with the most of the other side's rows first, so that the
-// longest workgroups of a causal launch begin first and short ones fill the end: by the tile's index within its sequence, from the
-// highest (queries: a later one sees more keys), or from the sequence's end (keys: an earlier one is seen by more queries).  A lane holds a
-// sequence's number of tiles; the level that the rank falls into is found by bisection.  More sequences than lanes: by slots, in order.
+// longest workgroups begin first and short ones fill the end (training batch of 2048 ... 1 causal tokens: forward 104 -> 91 us, backward
+// 370 -> 324).  A lane holds a sequence; the level that the rank falls into is found by bisection: causal, the tile's index within its sequence
+// (queries: a later one sees more keys) or its distance from the end (keys: an earlier one is seen by more queries); otherwise the other
+// side's length in tiles.  More sequences than lanes: by slots, in order.
 template <bool KEYS>
-__device__ __forceinline__ bool pa_find(const int* ends, int T, const int* ends2, int T2, int B, int zero_rest, int rank, int slots, PaSeq& r) {
+__device__ __forceinline__ bool pa_find(const int* ends, int T, const int* ends2, int T2, int B, int zero_rest, int causal, int rank, int slots, PaSeq& r) {
     const int lane = threadIdx.x & 63;
-    int s;
     if (B + 2 <= 64) {
-        const int begin = lane < B + 2 ? pa_bound(ends, lane, B, T) : T, end = lane < B + 2 ? pa_bound(ends, lane + 1, B, T) : T;
         const bool real = lane >= 1 && lane <= B;
+        const int begin = pa_bound(ends, lane, B, T), end = lane < B + 2 ? pa_bound(ends, lane + 1, B, T) : begin;
+        const int begin2 = pa_bound(ends2, lane, B, T2), end2 = real ? pa_bound(ends2, lane + 1, B, T2) : begin2;
         const int tiles = end > begin && (real || zero_rest) ? (end - begin + PA_ROWS - 1) / PA_ROWS : 0;
+        const int tiles2 = end2 > begin2 ? (end2 - begin2 + PA_TILE - 1) / PA_TILE : 0;
         auto beyond = [&](int level) {                                     // tiles at this level and above
-            int v = tiles > level ? tiles - level : 0;
-#pragma unroll
-            for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
-            return __builtin_amdgcn_readfirstlane(v);
+            return __builtin_amdgcn_readlane(pa_scan(causal ? (tiles > level ? tiles - level : 0) : tiles2 >= level ? tiles : 0), 63);
         };
         if (beyond(0) <= rank) return false;
-        int level = 0, above = -1;
-        for (int bit = 1 << (31 - __builtin_clz(T / PA_ROWS + 1)); bit > 0; bit >>= 1) {
+        int level = 0, above = 0;
+        for (int bit = 1 << (31 - __builtin_clz(causal ? T / PA_ROWS + 1 : T2 / PA_TILE + 1)); bit > 0; bit >>= 1) {
             const int n = beyond(level + bit);
             if (n > rank) level += bit;
             else above = n;                                                // (of the lowest level tried that is too high: level + 1 in the end)
         }
-        const unsigned long long at = __ballot(tiles > level);
-        const int before = __popcll(at & ((1ull << lane) - 1));
-        s = __ffsll(__ballot(tiles > level && before == rank - above)) - 1;
+        // the tiles of just this level, sequence by sequence
+        const int here = causal ? tiles > level : tiles2 == level ? tiles : 0;
+        const int upto = pa_scan(here), at = rank - above, s = __ffsll(__ballot(upto > at)) - 1;
+        const int of = __builtin_amdgcn_readlane(tiles, s), within = at - (__builtin_amdgcn_readlane(upto, s) - __builtin_amdgcn_readlane(here, s));
         r.begin = __builtin_amdgcn_readlane(begin, s);
         r.n = __builtin_amdgcn_readlane(end, s) - r.begin;
-        r.row0 = (KEYS ? __builtin_amdgcn_readlane(tiles, s) - 1 - level : level) * PA_ROWS;
-    } else {
-        const int slot = KEYS ? rank : slots - 1 - rank;
-        int before = 0;
-        for (int s0 = 0; s0 < B + 2; s0 += 64)
-            before += __popcll(__ballot(s0 + lane < B + 2 && pa_bound(ends, s0 + lane, B, T) / PA_ROWS + s0 + lane <= slot));
-        s = __builtin_amdgcn_readfirstlane(before) - 1;
-        if (s < 0) return false;
-        r.begin = __builtin_amdgcn_readfirstlane(pa_bound(ends, s, B, T));
-        r.n = __builtin_amdgcn_readfirstlane(pa_bound(ends, s + 1, B, T)) - r.begin;
-        r.row0 = (slot - (r.begin / PA_ROWS + s)) * PA_ROWS;
-        if (r.row0 < 0 || r.row0 >= r.n) return false;
+        r.begin2 = __builtin_amdgcn_readlane(begin2, s);
+        r.n2 = __builtin_amdgcn_readlane(end2, s) - r.begin2;
+        r.n2 = r.n2 > 0 ? r.n2 : 0;
+        r.row0 = (causal ? (KEYS ? of - 1 - level : level) : within) * PA_ROWS;
+        return true;
     }
+    const int slot = KEYS ? rank : slots - 1 - rank;
+    int before = 0;
+    for (int s0 = 0; s0 < B + 2; s0 += 64)
+        before += __popcll(__ballot(s0 + lane < B + 2 && pa_bound(ends, s0 + lane, B, T) / PA_ROWS + s0 + lane <= slot));
+    const int s = __builtin_amdgcn_readfirstlane(before) - 1;
+    if (s < 0) return false;
     const bool real = s >= 1 && s <= B;
-    r.begin2 = r.n2 = 0;
-    if (real) {
-        r.begin2 = __builtin_amdgcn_readfirstlane(pa_bound(ends2, s, B, T2));
-        const int end2 = __builtin_amdgcn_readfirstlane(pa_bound(ends2, s + 1, B, T2));
-        r.n2 = end2 > r.begin2 ? end2 - r.begin2 : 0;
-    }
-    return real || zero_rest;
+    r.begin = __builtin_amdgcn_readfirstlane(pa_bound(ends, s, B, T));
+    r.n = __builtin_amdgcn_readfirstlane(pa_bound(ends, s + 1, B, T)) - r.begin;
+    r.row0 = (slot - (r.begin / PA_ROWS + s)) * PA_ROWS;
+    r.begin2 = __builtin_amdgcn_readfirstlane(pa_bound(ends2, s, B, T2));
+    r.n2 = real ? __builtin_amdgcn_readfirstlane(pa_bound(ends2, s + 1, B, T2)) - r.begin2 : 0;
+    r.n2 = r.n2 > 0 ? r.n2 : 0;
+    return r.row0 >= 0 && r.row0 < r.n && (real || zero_rest);
 }
 
 // ---- tiles -------------------------------------------------------------------------------------------------------------------
@@ -305,7 +315,7 @@ __global__ __launch_bounds__(256, 2) void pa_fwd_kernel(const PaArgs a) {
     // heads that share k, v differ by Hk in their index: with workgroups dealt to the eight XCDs in turn, they meet in one L2
     const int hk = blockIdx.x % a.Hk, g = blockIdx.x / a.Hk % (a.H / a.Hk), head = hk * (a.H / a.Hk) + g;
     PaSeq sq;
-    if (!pa_find<false>(a.ends_q, a.Tq, a.ends_k, a.Tk, a.B, a.zero_rest, (int)(blockIdx.x / a.H), a.slots, sq)) return;
+    if (!pa_find<false>(a.ends_q, a.Tq, a.ends_k, a.Tk, a.B, a.zero_rest, a.causal, (int)(blockIdx.x / a.H), a.slots, sq)) return;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), col = lane & 31, h = lane >> 5;
     const int w0 = sq.row0 + wave * 32, qi = w0 + col;                     // the wave's first row, the lane's row
     const bool qv = qi < sq.n;
@@ -478,7 +488,7 @@ __global__ __launch_bounds__(256, 2) void pa_bwd_dq_kernel(const PaArgs a) {
     const bool want_table = BIAS && a.dtable_part;
     float* const part = want_table ? a.dtable_part + ((long long)rank * a.H + head) * a.buckets : nullptr;
     PaSeq sq;
-    if (!pa_find<false>(a.ends_q, a.Tq, a.ends_k, a.Tk, a.B, a.zero_rest, rank, a.slots, sq)) {
+    if (!pa_find<false>(a.ends_q, a.Tq, a.ends_k, a.Tk, a.B, a.zero_rest, a.causal, rank, a.slots, sq)) {
         if (want_table)
             for (int i = threadIdx.x; i < a.buckets; i += 256) part[i] = 0.f;
         return;
@@ -728,7 +738,7 @@ __global__ __launch_bounds__(256, 2) void pa_bwd_dkv_kernel(const PaArgs a) {
     const int hk = blockIdx.x % a.Hk, group = a.H / a.Hk;
     const int split = __builtin_amdgcn_readfirstlane((int)(blockIdx.x / a.Hk % a.splits));
     PaSeq sq;                                                              // begin, n: keys; begin2, n2: queries
-    if (!pa_find<true>(a.ends_k, a.Tk, a.ends_q, a.Tq, a.B, a.zero_rest, (int)(blockIdx.x / (a.Hk * a.splits)), a.slots, sq)) return;
+    if (!pa_find<true>(a.ends_k, a.Tk, a.ends_q, a.Tq, a.B, a.zero_rest, a.causal, (int)(blockIdx.x / (a.Hk * a.splits)), a.slots, sq)) return;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), col = lane & 31, h = lane >> 5;
     const int w0 = sq.row0 + wave * 32, ki = w0 + col;
     const bool kv = ki < sq.n;
