@@ -956,17 +956,17 @@ int pa_launch_bwd(PaArgs a, float* dtable, hipStream_t st) {
 }
 
 // How many workgroups share the queries of 128 keys.  The host knows sizes, not lengths: `groups` of keys, and on average `steps` tiles of
-// queries for each.  Two workgroups fit on a CU and those of a causal launch differ in length, so that about four for each CU are wanted; but each
-// share is written and read once more in 32 bits, and begins with k, v.  Backward pass in us, one share against the rule's:
-//   336 groups of 74 steps (causal, 128 wide)  562 / 370 (3)      544 of 256 (causal, 128 wide)  1327 / 974 (2)     112 of 44 (causal, 64 wide)  163 / 72 (9)
-//   18 of 16 (64 wide)                          80 / 31 (8)       268 of 128 (64 wide)            446 / 328 (3)
-// and where it leaves one, against two:  512 of 19 (64 wide) 136 / 147,  176 of 8 (causal, 64 wide) 36 / 41,  4288 of 64 (causal, 128 wide) 1962 / 2337.
+// queries for each.  Two workgroups fit on a CU, and more than one for each of the 512 places evens them out; but each share is written and
+// read once more in 32 bits, and begins with k, v.  Backward pass in us, one share against the rule's:
+//   336 groups of 74 steps (causal, 128 wide)  532 / 329 (3)      544 of 256 (causal, 128 wide)  1293 / 995 (2)     112 of 44 (causal, 64 wide)  161 / 72 (7)
+//   18 of 16 (64 wide)                          81 / 32 (8)       268 of 128 (64 wide)            447 / 335 (3)
+// and where it leaves one, against two:  512 of 19 (64 wide) 137 / 145,  176 of 8 (causal, 64 wide) 38 / 41,  4288 of 64 (causal, 128 wide) 2100 / 2589.
 int pa_splits(const ddpm_packed_attn_desc* d) {
     const long long groups = (long long)(d->Tk / PA_ROWS + d->B + 2) * d->Hk, steps = (long long)d->Tq / PA_TILE * (d->H / d->Hk) / (d->B > 0 ? d->B : 1);
     const long long most = steps / (groups >= 128 ? 16 : 2);               // (half of the card idle: even short shares pay)
-    long long z = 1100 / groups;
+    long long z = (700 + groups - 1) / groups;
     z = z < most ? z : most;
-    return z < 1 ? 1 : z > 12 ? 12 : (int)z;
+    return z < 1 ? 1 : z > 8 ? 8 : (int)z;
 }
 
 template <typename F> int pa_dispatch(const ddpm_packed_attn_desc* d, F&& f) {
