@@ -104,7 +104,7 @@ __device__ __forceinline__ void group_finish(int tid, const float* s_part, float
         }
         const float im = 1.0f / (float)(E::CPG * HW);
         const float mean = S * im;
-        const float var = fmaxf(SS * im - mean * mean, 0.f);
+        const float var = fmaxf(fmaf(-mean, mean, SS * im), 0.f);      // one rounding order whatever the compiler contracts
         const float rstd = rsqrtf(var + eps);
         s_mr[tid * 2] = mean; s_mr[tid * 2 + 1] = rstd;
         if (st_out && n0 + img < N) {
