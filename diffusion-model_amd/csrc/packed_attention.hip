@@ -291,12 +291,16 @@ template <typename T> __device__ __forceinline__ typename PaTypes<T>::v8 pa_pack
 }
 
 // ---- relative position bias ----------------------------------------------------------------------------------------------------
-// LDS: the bias of every distance key - query in -far ... far for one head, in units of log2 like the scores.
+// LDS: the bias of every distance key - query in -far ... far for one head, in units of log2 like the scores.  Finite ones are limited to
+// PA_MAX_BIAS: a row all of whose keys have the same large bias keeps its scores and its normaliser in 32 bits (with a bias of -1e9 both
+// would be lost, and the backward pass could not rebuild the probabilities).  -inf stays: a distance that is not seen.
+#define PA_MAX_BIAS 8192.f
 __device__ __forceinline__ void pa_bias_fill(const PaArgs& a, int head, float* s_bias) {
     for (int i = threadIdx.x; i < 2 * a.far + 1; i += blockDim.x) {
         int b = a.bucket_of[i];
         b = b < 0 ? 0 : b >= a.buckets ? a.buckets - 1 : b;
-        s_bias[i] = a.table[b * a.H + head] * 1.4426950408889634f;
+        const float x = a.table[b * a.H + head] * 1.4426950408889634f;
+        s_bias[i] = fabsf(a.table[b * a.H + head]) < INFINITY ? fminf(fmaxf(x, -PA_MAX_BIAS), PA_MAX_BIAS) : x;
     }
 }
 __device__ __forceinline__ int pa_clamp(int d, int far) { return d < -far ? -far : d > far ? far : d; }
@@ -722,7 +726,8 @@ __global__ __launch_bounds__(256) void pa_dtable_kernel(const float* __restrict_
 // backward: dk, dv; a wave owns 32 keys and walks over the queries of every head that shares them
 // ================================================================================================================================
 // Heads of 128: the accumulators and k take 160 registers, so that v is read from LDS and tiles are 32 queries, which leaves room for two
-// workgroups on a CU, each waiting at barriers of its own (v in registers: one workgroup, LATER).
+// workgroups on a CU, each waiting at barriers of its own (v in registers and tiles of 64 queries, one workgroup: 409 us against 240 for the batch of 2048 ... 1
+// causal tokens, 16 heads over 4).
 // The steps (heads of the group x tiles of queries) may be split over several workgroups, whose 32-bit sums a last launch adds
 // up: few keys with long sequences and shared heads would leave most of the card idle otherwise.
 template <typename T, int DHP, bool BIAS>
@@ -996,7 +1001,8 @@ int pa_setup(const ddpm_packed_attn_desc* d, bool bwd, PaArgs& a) {
     DDPM_REQUIRE(d->Tq >= 0 && d->Tk >= 0 && d->B >= 0 && d->Tq < (1 << 30) && d->Tk < (1 << 30) && d->B < (1 << 24), "packed_attention: %d queries, %d keys, %d sequences", d->Tq, d->Tk, d->B);
     DDPM_REQUIRE(d->ends_q && d->ends_k, "packed_attention: the sequences' boundaries are missing");
     DDPM_REQUIRE(d->scale > 0.f && d->scale < INFINITY, "packed_attention: scale must be positive and finite");
-    DDPM_REQUIRE((int64_t)(d->Tq / PA_ROWS + d->B + 2) * d->H < (1ll << 31) && (int64_t)(d->Tk / PA_ROWS + d->B + 2) * d->Hk < (1ll << 31), "packed_attention: too many workgroups");
+    // (a launch is limited to 2^32 - 1 threads)
+    DDPM_REQUIRE((int64_t)(d->Tq / PA_ROWS + d->B + 2) * d->H < (1ll << 24) && (int64_t)(d->Tk / PA_ROWS + d->B + 2) * d->Hk < (1ll << 24), "packed_attention: too many workgroups");
     DDPM_REQUIRE(!d->table == !d->bucket_of, "packed_attention: the bias needs both its table and the buckets of the distances");
     a = {};
     if (d->table) {

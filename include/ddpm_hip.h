@@ -612,6 +612,7 @@ int ddpm_adam_step_clipped(float* p, const float* g, float* m, float* v, float* 
  * DDPM_F16); strides are multiples of 8, base pointers 16-byte aligned, dh a multiple of 8 up to 128.
  * Bias: table fp32 [buckets][H], bucket_of int32 [2 far + 1] (device): the bucket of the distance key - query (the query's place
  * counted from the sequence's end when causal: i + keys - queries) clamped to -far .. far; 4 <= far <= 1024.  Both NULL: no bias.
+ * A table entry of -inf hides its distances; finite ones beyond +-8192 / log2(e) count as that.
  * Rows outside of all sequences: zeros in o (dq, dk, dv) with zero_rest != 0, left as they were otherwise.
  * lse fp32 [H][Tq] (base-2 log-sum-exp, -inf without a key) and o32 fp32 [Tq][H][dh] (o before rounding) are written by forward when
  * not NULL (o32 of a launch with a bias is computed from probabilities in two 16-bit parts, i.e. to about 2^-16); backward reads lse, and

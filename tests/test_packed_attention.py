@@ -172,6 +172,30 @@ def test_large_scores_and_bias(dev):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("causal", [False, True])
+@pytest.mark.parametrize("heads,kv,width,table", [(2, 1, 64, (8, 16, True)), (2, 2, 128, (32, 1024, True))])
+def test_a_bias_of_the_lowest_value(dev, causal, heads, kv, width, table):
+    """float32's lowest value, -1e9 and 1e6 as biases, for one bucket and for all of them (the rows' keys are then masked alike and keep their
+    scores): as biases of +-8192 / log2(e), which is where the kernels limit them"""
+    limit = 8192 * math.log(2.0)
+    for low in (torch.finfo(torch.float32).min, -1e9):
+        for rows in (slice(0, 1), slice(2, 5), slice(None)):
+            d = make([200, 1, 70], [200, 1, 70], heads, kv, width, torch.bfloat16, seed=18, table=table)
+            d["table"][rows] = low
+            got = run(d, dev, causal, cross=False)
+            d["table"].clamp_(-limit, limit)
+            want, tol = reference(d, causal)
+            for n in want:
+                check(n, got[n], want[n], tol[n])
+    d["table"][:] = 1e6
+    got = run(d, dev, causal, cross=False)
+    d["table"][:] = limit
+    want, tol = reference(d, causal)
+    for n in want:
+        check(n, got[n], want[n], tol[n])
+
+
+@pytest.mark.gpu
 def test_infinities_and_nan_outside_stay_there(dev):
     """NaN in rows of no sequence and in another sequence; -inf and inf where the mask hides them"""
     d = make([40, 90], [40, 90], 2, 1, 64, torch.bfloat16, seed=9, tail=6)
@@ -187,6 +211,21 @@ def test_infinities_and_nan_outside_stay_there(dev):
     got = run(d, dev, False, cross=False)
     for n in ("o", "dq", "dk", "dv"):
         assert torch.equal(got[n][:40], clean[n][:40]), n
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("width", [8, 32, 64, 128])
+@pytest.mark.parametrize("causal", [False, True])
+def test_a_tile_ends_where_its_sequence_does(dev, width, causal):
+    """NaN in every row behind a sequence that ends inside a tile, at every load of the tile: nothing of it arrives, not even times zero"""
+    for n in (1, 3, 5, 9, 17, 31, 33, 50, 63, 65, 100):
+        d = make([n, 140], [n, 140], 4, 2, width, torch.bfloat16, seed=n)
+        clean = run(d, dev, causal, cross=False)
+        for name in ("q", "k", "v", "do"):
+            d[name][n:] = math.nan
+        got = run(d, dev, causal, cross=False)
+        for name in ("o", "dq", "dk", "dv"):
+            assert torch.equal(got[name][:n], clean[name][:n]), (n, name)
 
 
 @pytest.mark.gpu
@@ -394,7 +433,7 @@ def test_refusals_without_a_gpu():
                      (dict(ends_q=None), b"boundaries"), (dict(q=None), b"q is null"), (dict(v=at + 2), b"16-byte"), (dict(k_row=252), b"strides of k"), (dict(o_head=0), b"strides of o"),
                      (dict(q_row=1 << 24), b"2^24"), (dict(k_head=32), b"shorter"), (dict(table=at), b"both"), (dict(table=at, bucket_of=at, far=3, buckets=8), b"distances"),
                      (dict(table=at, bucket_of=at, far=1025, buckets=8), b"distances"), (dict(table=at, bucket_of=at, far=8, buckets=0), b"buckets"),
-                     (dict(B=(1 << 24) - 1, H=1024), b"workgroups")):
+                     (dict(B=(1 << 24) - 1, H=1024), b"workgroups"), (dict(B=1 << 22), b"workgroups")):
         assert hip.lib().ddpm_packed_attention_forward(ctypes.byref(hip.PackedAttnDesc(**dict(good, **bad))), None) != 0 and why in last(), (bad, last())
     for bad, why in ((dict(lse=None), b"lse"), (dict(dsum=None), b"dsum"), (dict(dtable=at), b"not there"), (dict(table=at, bucket_of=at, far=8, buckets=8, dtable=at), b"dtable_part"),
                      (dict(dq=at + 8), b"dq"), (dict(dout_row=100), b"dout")):
