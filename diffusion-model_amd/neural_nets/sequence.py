@@ -5,13 +5,14 @@ everywhere in this package.  The reference has no such encoder; its ConditionalM
 (constituent_blocks.py:402-437 there)."""
 from __future__ import annotations
 
+import weakref
 from typing import Optional
 
 import torch
 from torch import Tensor, nn
 from torch.autograd.function import once_differentiable
 
-from ..runtime import ops
+from ..runtime import hip, ops
 
 
 def _need_gpu(what: str, *tensors) -> None:
@@ -35,17 +36,51 @@ def _rows(t: Tensor, c: int) -> Tensor:
     return r if r.stride(1) == 1 else r.as_strided(r.shape, (1, 1))         # (c = 1: torch leaves such a stride as it was)
 
 
+class _LeafUse:
+    """A leaf that autograd graphs of this module use: alive as long as one of those graphs is"""
+    __slots__ = ("leaf", "stream", "__weakref__")
+
+    def __init__(self, leaf: Tensor, stream: int):
+        self.leaf, self.stream = weakref.ref(leaf), stream
+
+
+_leaf_uses: "weakref.WeakValueDictionary[int, _LeafUse]" = weakref.WeakValueDictionary()
+
+
+def _note_leaves(ctx, *inputs) -> None:
+    """All graphs of a leaf share the node that receives its gradient, and that node stays with the stream of the graph that made it.  If that is
+    the default stream, autograd makes it wait for a captured backward pass, which no capture survives (nor does the process): so
+    the backward pass of a captured graph looks for such a graph, and refuses in time."""
+    capturing, ctx.stale, ctx.uses = torch.cuda.is_current_stream_capturing(), False, []
+    for t in inputs:
+        if t is not None and t.requires_grad and t.is_leaf:
+            use = _leaf_uses.get(id(t))
+            if use is None or use.leaf() is not t:
+                use = _leaf_uses[id(t)] = _LeafUse(t, hip.stream())
+            elif capturing and use.stream == 0:
+                ctx.stale = True
+            ctx.uses.append(use)
+
+
+def _refuse_stale(ctx, what: str) -> None:
+    if ctx.stale and torch.cuda.is_current_stream_capturing():
+        raise RuntimeError(f"{what}: this backward pass is being captured while an earlier graph of the same parameters or inputs, made on the default "
+                           "stream, is alive; delete its results (or make it on a side stream) before the capture")
+
+
 class _LayerNormFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x: Tensor, weight: Optional[Tensor], bias: Optional[Tensor], eps: float):
         rows = _rows(x, x.shape[-1])
         y, stats = ops.layer_norm_forward(rows, weight, bias, eps, want_stats=any(ctx.needs_input_grad))
+        _note_leaves(ctx, x, weight, bias)
         ctx.save_for_backward(rows, weight, stats)
         return y.view(x.shape)
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dy: Tensor):
+        _refuse_stale(ctx, "layer_norm")
         rows, weight, stats = ctx.saved_tensors
         nx, nw, nb, _ = ctx.needs_input_grad
         dx, dw, db = ops.layer_norm_backward(rows, _rows(dy, rows.shape[1]), weight, stats, want_dx=nx, want_dw=nw, want_db=nb)
@@ -90,6 +125,7 @@ def _heads(t: Tensor) -> Tensor:
 class _PackedAttentionFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, table, ends_q, ends_k, bucket_of, causal: bool, scale: Optional[float]):
+        _note_leaves(ctx, q, k, v, table)
         q, k, v = _heads(q), _heads(k), _heads(v)
         train = any(ctx.needs_input_grad)
         o, lse, o32 = ops.packed_attention_forward(q, k, v, ends_q, ends_k, causal=causal, scale=scale, table=table, bucket_of=bucket_of,
@@ -101,6 +137,7 @@ class _PackedAttentionFn(torch.autograd.Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, dout: Tensor):
+        _refuse_stale(ctx, "packed_attention")
         q, k, v, table, ends_q, ends_k, bucket_of, o, lse, o32 = ctx.saved_tensors
         dq, dk, dv, dtable = ops.packed_attention_backward(q, k, v, o, lse, _heads(dout), ends_q, ends_k, causal=ctx.how[0], scale=ctx.how[1], table=table,
                                                            bucket_of=bucket_of, o32=o32, want_dtable=o32 is not None)
@@ -119,7 +156,8 @@ def packed_attention(q: Tensor, k: Tensor, v: Tensor, ends: Tensor, *, ends_k: O
     causal: a query sees the keys up to its own place, counted from the sequences' ends where there are more or fewer keys than queries.
     A query that sees no key gets zeros.
     bias_table [buckets, heads] (fp32, learned) with bias_buckets [2 far + 1] (int32, relative_position_buckets): adds
-    bias_table[bucket of (key's place - query's place), head] to the score.
+    bias_table[bucket of (key's place - query's place), head] to the score.  A bias of -inf hides its distances; finite ones beyond +-5678
+    (2^13 powers of two) count as that.
     Differentiable once in q, k, v and bias_table."""
     for name, t in (("q", q), ("k", k), ("v", v)):
         if t.dim() != 3:

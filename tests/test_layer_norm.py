@@ -166,6 +166,33 @@ def test_layer_norm_module_and_graph(dev):
             assert torch.equal(a, b), k
 
 
+@pytest.mark.gpu
+def test_capture_beside_a_living_graph_is_refused(dev):
+    """a graph of the same parameters that an eager call on the default stream made and that is still alive: a captured backward pass would
+    make the default stream wait for the capture.  It is refused before that; without the graph it goes through"""
+    m = sequence.LayerNorm(64, device=dev)
+    x = torch.randn(8, 64, device=dev)
+    old = m(x)
+    assert not torch.cuda.is_current_stream_capturing()
+    with torch.no_grad():                                                         # (a capture without a backward pass is free to go on)
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            m(x)
+    with pytest.raises(RuntimeError, match="is alive"):
+        with torch.cuda.graph(torch.cuda.CUDAGraph()):
+            torch.autograd.grad(m(x), [m.weight, m.bias], x)
+    torch.cuda.synchronize()
+    want = torch.autograd.grad(old, [m.weight, m.bias], x)
+    del old
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        got = torch.autograd.grad(m(x), [m.weight, m.bias], x)
+    for _ in range(2):
+        g.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
 def test_layer_norm_refusals_without_a_gpu():
     with pytest.raises(RuntimeError, match="HIP kernels only"):
         sequence.layer_norm(torch.zeros(2, 8))
