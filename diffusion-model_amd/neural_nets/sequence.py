@@ -36,30 +36,22 @@ def _rows(t: Tensor, c: int) -> Tensor:
     return r if r.stride(1) == 1 else r.as_strided(r.shape, (1, 1))         # (c = 1: torch leaves such a stride as it was)
 
 
-class _LeafUse:
-    """A leaf that autograd graphs of this module use: alive as long as one of those graphs is"""
-    __slots__ = ("leaf", "stream", "__weakref__")
-
-    def __init__(self, leaf: Tensor, stream: int):
-        self.leaf, self.stream = weakref.ref(leaf), stream
+_graphs: list = []                   # weak references to the nodes of this module's autograd graphs, dead ones swept now and then
 
 
-_leaf_uses: "weakref.WeakValueDictionary[int, _LeafUse]" = weakref.WeakValueDictionary()
-
-
-def _note_leaves(ctx, *inputs) -> None:
+def _note_graph(ctx, *inputs) -> None:
     """All graphs of a leaf share the node that receives its gradient, and that node stays with the stream of the graph that made it.  If that is
     the default stream, autograd makes it wait for a captured backward pass, which no capture survives (nor does the process): so
     the backward pass of a captured graph looks for such a graph, and refuses in time."""
-    capturing, ctx.stale, ctx.uses = torch.cuda.is_current_stream_capturing(), False, []
-    for t in inputs:
-        if t is not None and t.requires_grad and t.is_leaf:
-            use = _leaf_uses.get(id(t))
-            if use is None or use.leaf() is not t:
-                use = _leaf_uses[id(t)] = _LeafUse(t, hip.stream())
-            elif capturing and use.stream == 0:
-                ctx.stale = True
-            ctx.uses.append(use)
+    ctx.stream, ctx.stale = hip.stream(), False
+    if ctx.stream == 0:
+        _graphs.append(weakref.ref(ctx))
+        if len(_graphs) >= 4096:
+            _graphs[:] = [r for r in _graphs if r() is not None]
+    elif torch.cuda.is_current_stream_capturing():
+        leaves = [t for t in inputs if t is not None and t.requires_grad and t.is_leaf]
+        held = [getattr(node, "variable", None) for r in _graphs if (graph := r()) is not None for node, _ in graph.next_functions]
+        ctx.stale = any(h is t for h in held if h is not None for t in leaves)
 
 
 def _refuse_stale(ctx, what: str) -> None:
@@ -73,7 +65,7 @@ class _LayerNormFn(torch.autograd.Function):
     def forward(ctx, x: Tensor, weight: Optional[Tensor], bias: Optional[Tensor], eps: float):
         rows = _rows(x, x.shape[-1])
         y, stats = ops.layer_norm_forward(rows, weight, bias, eps, want_stats=any(ctx.needs_input_grad))
-        _note_leaves(ctx, x, weight, bias)
+        _note_graph(ctx, x, weight, bias)
         ctx.save_for_backward(rows, weight, stats)
         return y.view(x.shape)
 
@@ -125,7 +117,7 @@ def _heads(t: Tensor) -> Tensor:
 class _PackedAttentionFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, table, ends_q, ends_k, bucket_of, causal: bool, scale: Optional[float]):
-        _note_leaves(ctx, q, k, v, table)
+        _note_graph(ctx, q, k, v, table)
         q, k, v = _heads(q), _heads(k), _heads(v)
         train = any(ctx.needs_input_grad)
         o, lse, o32 = ops.packed_attention_forward(q, k, v, ends_q, ends_k, causal=causal, scale=scale, table=table, bucket_of=bucket_of,
