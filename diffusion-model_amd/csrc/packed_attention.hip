@@ -348,7 +348,16 @@ __global__ __launch_bounds__(256, 2) void pa_fwd_kernel(const PaArgs a) {
     };
     if (tiles > 0) fetch(0);
     unsigned rp = pa_row_place<DHP>(col, h), cp = pa_col_place<DHP>();
-    for (int t = 0; t < tiles; ++t) {
+    const int seen = a.causal ? w0 + w_rows - 1 + off : sq.n2 - 1;         // the last key that a row of the wave sees
+    const int mine = w_rows > 0 && seen >= 0 ? (seen / PA_TILE + 1 < tiles ? seen / PA_TILE + 1 : tiles) : 0;
+    auto arrive = [&](int t) {
+        pa_arrived();
+        __syncthreads();                                                   // this tile is there, and the one before it has been read
+        if (t + 1 < tiles) fetch(t + 1);
+    };
+    // (tiles that the wave has no part in, all behind its own, have a loop of their own: as a branch in this one they made the compiler move the
+    // accumulators to other registers and back for every tile, 64 instructions; 1067 -> 1022 us for 16 K causal tokens)
+    for (int t = 0; t < mine; ++t) {
         if (BIAS) {
             pa_opaque<DHP>(rp);
             pa_opaque<DHP>(cp);
@@ -356,93 +365,90 @@ __global__ __launch_bounds__(256, 2) void pa_fwd_kernel(const PaArgs a) {
         const char* const lk = smem + (t & 1) * 2 * TL::BYTES;
         const char* const lv = lk + TL::BYTES;
         const int k0 = t * PA_TILE;
-        pa_arrived();
-        __syncthreads();                                                   // this tile is there, and the one before it has been read
-        if (t + 1 < tiles) fetch(t + 1);
-        if (w_rows > 0 && (!a.causal || k0 <= w0 + w_rows - 1 + off)) {
-            f32x16 sc[2] = {pa_zero(), pa_zero()};
-            __builtin_amdgcn_s_setprio(1);
+        arrive(t);
+        f32x16 sc[2] = {pa_zero(), pa_zero()};
+        __builtin_amdgcn_s_setprio(1);
 #pragma unroll
-            for (int kc = 0; kc < KC; ++kc) {
-                sc[0] = pa_mfma(pa_row_frag<v8, DHP>(lk, rp, kc), bq[kc], sc[0]);
-                sc[1] = pa_mfma(pa_row_frag<v8, DHP>(lk + 32 * TL::RB, rp, kc), bq[kc], sc[1]);
-            }
-            pa_order<2 * KC, 1, 4>();
-            __builtin_amdgcn_s_setprio(0);
-            float s[32];
-            const int dist0 = k0 + h * 4 - (qi + off);                     // distance of the lane's first score
-            if (BIAS) {
-                const int lo = k0 - (w0 + 31 + off), hi = k0 + PA_TILE - 1 - (w0 + off);       // distances in the wave's tile
-                if (hi <= -a.far || lo >= a.far) {
-                    const float b = s_bias[hi <= -a.far ? 0 : 2 * a.far];
+        for (int kc = 0; kc < KC; ++kc) {
+            sc[0] = pa_mfma(pa_row_frag<v8, DHP>(lk, rp, kc), bq[kc], sc[0]);
+            sc[1] = pa_mfma(pa_row_frag<v8, DHP>(lk + 32 * TL::RB, rp, kc), bq[kc], sc[1]);
+        }
+        pa_order<2 * KC, 1, 4>();
+        __builtin_amdgcn_s_setprio(0);
+        float s[32];
+        const int dist0 = k0 + h * 4 - (qi + off);                     // distance of the lane's first score
+        if (BIAS) {
+            const int lo = k0 - (w0 + 31 + off), hi = k0 + PA_TILE - 1 - (w0 + off);       // distances in the wave's tile
+            if (hi <= -a.far || lo >= a.far) {
+                const float b = s_bias[hi <= -a.far ? 0 : 2 * a.far];
 #pragma unroll
-                    for (int i = 0; i < 32; ++i) s[i] = sc[i >> 4][i & 15] * a.scale2 + b;
-                } else if (lo > -a.far && hi < a.far) {                    // no distance is clamped: one address, constant offsets
-                    const float* const b = s_bias + dist0 + a.far;
+                for (int i = 0; i < 32; ++i) s[i] = sc[i >> 4][i & 15] * a.scale2 + b;
+            } else if (lo > -a.far && hi < a.far) {                    // no distance is clamped: one address, constant offsets
+                const float* const b = s_bias + dist0 + a.far;
 #pragma unroll
-                    for (int i = 0; i < 32; ++i) s[i] = sc[i >> 4][i & 15] * a.scale2 + b[(i >> 2) * 8 + (i & 3)];
-                } else {
-#pragma unroll
-                    for (int i = 0; i < 32; ++i)
-                        s[i] = sc[i >> 4][i & 15] * a.scale2 + s_bias[pa_clamp(dist0 + (i >> 2) * 8 + (i & 3), a.far) + a.far];
-                }
+                for (int i = 0; i < 32; ++i) s[i] = sc[i >> 4][i & 15] * a.scale2 + b[(i >> 2) * 8 + (i & 3)];
             } else {
 #pragma unroll
-                for (int i = 0; i < 32; ++i) s[i] = sc[i >> 4][i & 15];    // (scaled where the maximum is subtracted, in one instruction)
+                for (int i = 0; i < 32; ++i)
+                    s[i] = sc[i >> 4][i & 15] * a.scale2 + s_bias[pa_clamp(dist0 + (i >> 2) * 8 + (i & 3), a.far) + a.far];
             }
-            if (k0 + PA_TILE > sq.n2 || (a.causal && k0 + PA_TILE - 1 > w0 + off)) {
-                // key index - k0 of score i is (i >> 2) * 8 + h * 4 + (i & 3): beyond `last` it is not seen
-                const int last = (a.causal && qi + off < sq.n2 - 1 ? qi + off : sq.n2 - 1) - k0 - h * 4;
+        } else {
 #pragma unroll
-                for (int i = 0; i < 32; ++i) s[i] = (i >> 2) * 8 + (i & 3) <= last ? s[i] : -INFINITY;
-            }
-            const float unit = BIAS ? 1.f : a.scale2;                      // (positive: the maximum may be taken before)
-            float mx = s[0];
-#pragma unroll
-            for (int i = 1; i < 32; ++i) mx = fmaxf(mx, s[i]);
-            mx = pa_half_max(mx) * unit;
-            // The maximum moves only when a row's grows by more than 2^8: until then the old one keeps every term below 2^8, which
-            // costs no precision, and the accumulators need no rescaling.
-            if (__any(mx > m + 8.f)) {
-                const float mn = fmaxf(m, mx), ref = mn == -INFINITY ? 0.f : mn;       // (a row that has seen nothing yet stays at zero)
-                const float alpha = __builtin_amdgcn_exp2f(m - ref);
-                l *= alpha;
-                m = mn;
-#pragma unroll
-                for (int mt = 0; mt < MT; ++mt)
-#pragma unroll
-                    for (int i = 0; i < 16; ++i) acc[mt][i] *= alpha;
-            }
-            const float ref = m == -INFINITY ? 0.f : m;
-            float sum = 0.f;
-#pragma unroll
-            for (int i = 0; i < 32; ++i) {
-                s[i] = __builtin_amdgcn_exp2f(s[i] * unit - ref);
-                sum += s[i];
-            }
-            l += sum;                                                      // (this half-wave's keys; joined at the end)
-            // p is rounded to the type of v for the product (relative 2^-8 of each term in bf16, of either sign); the sum above is not.
-            // Where the output feeds the bias's gradient, whose terms cancel, what that rounding leaves is multiplied as well.
-            __builtin_amdgcn_s_setprio(1);
-#pragma unroll
-            for (int c = 0; c < 4; ++c) {
-                const v8 p = pa_pack<T>(s + 8 * c);
-                v8 rest;
-                if constexpr (TWO) {
-#pragma unroll
-                    for (int j = 0; j < 8; ++j) rest[j] = (T)(s[8 * c + j] - (float)p[j]);
-                }
-#pragma unroll
-                for (int mt = 0; mt < MT; ++mt) {
-                    const v8 f = pa_col_frag<v8, DHP>(lv, cp, 16 * c, mt);
-                    acc[mt] = pa_mfma(f, p, acc[mt]);
-                    if constexpr (TWO) acc[mt] = pa_mfma(f, rest, acc[mt]);
-                }
-            }
-            if (!TWO) pa_order<4 * MT, 2, 3>();
-            __builtin_amdgcn_s_setprio(0);
+            for (int i = 0; i < 32; ++i) s[i] = sc[i >> 4][i & 15];    // (scaled where the maximum is subtracted, in one instruction)
         }
+        if (k0 + PA_TILE > sq.n2 || (a.causal && k0 + PA_TILE - 1 > w0 + off)) {
+            // key index - k0 of score i is (i >> 2) * 8 + h * 4 + (i & 3): beyond `last` it is not seen
+            const int last = (a.causal && qi + off < sq.n2 - 1 ? qi + off : sq.n2 - 1) - k0 - h * 4;
+#pragma unroll
+            for (int i = 0; i < 32; ++i) s[i] = (i >> 2) * 8 + (i & 3) <= last ? s[i] : -INFINITY;
+        }
+        const float unit = BIAS ? 1.f : a.scale2;                      // (positive: the maximum may be taken before)
+        float mx = s[0];
+#pragma unroll
+        for (int i = 1; i < 32; ++i) mx = fmaxf(mx, s[i]);
+        mx = pa_half_max(mx) * unit;
+        // The maximum moves only when a row's grows by more than 2^8: until then the old one keeps every term below 2^8, which
+        // costs no precision, and the accumulators need no rescaling.
+        if (__any(mx > m + 8.f)) {
+            const float mn = fmaxf(m, mx), ref = mn == -INFINITY ? 0.f : mn;       // (a row that has seen nothing yet stays at zero)
+            const float alpha = __builtin_amdgcn_exp2f(m - ref);
+            l *= alpha;
+            m = mn;
+#pragma unroll
+            for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) acc[mt][i] *= alpha;
+        }
+        const float ref = m == -INFINITY ? 0.f : m;
+        float sum = 0.f;
+#pragma unroll
+        for (int i = 0; i < 32; ++i) {
+            s[i] = __builtin_amdgcn_exp2f(s[i] * unit - ref);
+            sum += s[i];
+        }
+        l += sum;                                                      // (this half-wave's keys; joined at the end)
+        // p is rounded to the type of v for the product (relative 2^-8 of each term in bf16, of either sign); the sum above is not.
+        // Where the output feeds the bias's gradient, whose terms cancel, what that rounding leaves is multiplied as well.
+        __builtin_amdgcn_s_setprio(1);
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+            const v8 p = pa_pack<T>(s + 8 * c);
+            v8 rest;
+            if constexpr (TWO) {
+#pragma unroll
+                for (int j = 0; j < 8; ++j) rest[j] = (T)(s[8 * c + j] - (float)p[j]);
+            }
+#pragma unroll
+            for (int mt = 0; mt < MT; ++mt) {
+                const v8 f = pa_col_frag<v8, DHP>(lv, cp, 16 * c, mt);
+                acc[mt] = pa_mfma(f, p, acc[mt]);
+                if constexpr (TWO) acc[mt] = pa_mfma(f, rest, acc[mt]);
+            }
+        }
+        if (!TWO) pa_order<4 * MT, 2, 3>();
+        __builtin_amdgcn_s_setprio(0);
     }
+    for (int t = mine; t < tiles; ++t) arrive(t);
     l = pa_half_sum(l);
     const float inv = l == 0.f ? 0.f : 1.f / l;
     pa_put<T, DHP>(acc, pa_rows(a.o, sq.begin + w0, w_rows, head, a.dh), [&](float x) { return x * inv; });
@@ -508,6 +514,8 @@ __global__ __launch_bounds__(256, 2) void pa_bwd_dq_kernel(const PaArgs a) {
             for (int i = threadIdx.x; i < 4 * width; i += 256) s_sum[i] = 0.f;
     }
     float* const my_sum = s_sum + wave * width, *const s_tile = s_sum + 4 * width + wave * (32 * 17);   // the tile: [query][key], 17 apart
+    // bit kk: the lane's diagonal has an element at key kk, 0 <= kk + 31 - lane <= 31
+    const int on_tile = lane <= 31 ? (2 << lane) - 1 : lane < 63 ? -1 << (lane - 31) : 0;
     float before = 0.f, after = 0.f, pbefore = 0.f, pafter = 0.f;          // ds and p at distances <= -far, >= far
     float all = 0.f;                                                       // every ds of the row
 
@@ -558,10 +566,10 @@ __global__ __launch_bounds__(256, 2) void pa_bwd_dq_kernel(const PaArgs a) {
         pa_load<DHP, PA_TILE>(to + TL::BYTES, vb, a.v.row, t * PA_TILE, sq.n2, a.dh, vo);
     };
     unsigned rp = pa_row_place<DHP>(col, h), cp = pa_col_place<DHP>();
-    // probabilities (zero where the key is not seen) and do . v of 32 keys
-    auto scores = [&](const char* lk, const char* lv, int sub, int k0, float (&p)[16], f32x16& dp) {
+    // probabilities (zero where the key is not seen) and from + do . v of 32 keys
+    auto scores = [&](const char* lk, const char* lv, int sub, int k0, float (&p)[16], f32x16& dp, const f32x16& from) {
         f32x16 sc = pa_zero();
-        dp = pa_zero();
+        dp = from;
         __builtin_amdgcn_s_setprio(1);
 #pragma unroll
         for (int kc = 0; kc < KC; ++kc) {
@@ -606,13 +614,16 @@ __global__ __launch_bounds__(256, 2) void pa_bwd_dq_kernel(const PaArgs a) {
             if (sees(u * 32)) {
                 float p[16];
                 f32x16 dp;
-                scores(lk, lk + TL::BYTES, u & 1, u * 32, p, dp);
+                scores(lk, lk + TL::BYTES, u & 1, u * 32, p, dp, pa_zero());
 #pragma unroll
                 for (int i = 0; i < 16; ++i) dsum += p[i] * dp[i];
             }
         }
         dsum = pa_half_sum(dsum);
     }
+    f32x16 minus_d;                                                        // do . v - D: the products begin with -D, sixteen registers that never change
+#pragma unroll
+    for (int i = 0; i < 16; ++i) minus_d[i] = -dsum;
     for (int t = 0; t < tiles; ++t) {
         const char* const lk = smem + (t & 1) * 2 * TL::BYTES;
         const char* const lv = lk + TL::BYTES;
@@ -629,10 +640,10 @@ __global__ __launch_bounds__(256, 2) void pa_bwd_dq_kernel(const PaArgs a) {
             if (sees(k0)) {
                 float p[16], ds[16], sum = 0.f;
                 f32x16 dp;
-                scores(lk, lv, sub, k0, p, dp);
+                scores(lk, lv, sub, k0, p, dp, minus_d);
 #pragma unroll
                 for (int i = 0; i < 16; ++i) {
-                    ds[i] = p[i] * (dp[i] - dsum);
+                    ds[i] = p[i] * dp[i];
                     sum += ds[i];
                 }
                 all += sum;
@@ -651,18 +662,18 @@ __global__ __launch_bounds__(256, 2) void pa_bwd_dq_kernel(const PaArgs a) {
 #pragma unroll
                             for (int i = 0; i < 8; ++i) s_tile[col * 17 + (i >> 2) * 8 + h * 4 + (i & 3)] = ds[half * 8 + i];
                             pa_wave_order();
-                            // lane's diagonal: key - query = lane - 31; what a lane reads off the tile's ends is dropped
+                            // lane's diagonal: key - query = lane - 31; what a lane reads off the tile's ends is dropped, by bits (as
+                            // conditions they became sixteen branches around sixteen reads that waited for each other)
                             const float* const at = s_tile + (31 - lane) * 17;
-                            float x = 0.f;
+                            float e[16], x = 0.f;
 #pragma unroll
-                            for (int kk = 0; kk < 16; ++kk) {
-                                const float e = at[kk * 18];
-                                x += kk <= lane && kk >= lane - 31 ? e : 0.f;
-                            }
+                            for (int kk = 0; kk < 16; ++kk) e[kk] = at[kk * 18];
+#pragma unroll
+                            for (int kk = 0; kk < 16; ++kk) x += __int_as_float(__float_as_int(e[kk]) & __builtin_amdgcn_sbfe(on_tile, kk, 1));
                             const int d = k0 + half * 16 - (w0 + off) + lane - 31;
-                            if (d <= -a.far) before += x;
-                            else if (d >= a.far) after += x;
-                            else if (lane < 47) my_sum[d + a.far] += x;
+                            before += d <= -a.far ? x : 0.f;
+                            after += d >= a.far ? x : 0.f;
+                            if (d > -a.far && d < a.far && lane < 47) my_sum[d + a.far] += x;
                         }
                     }
                 }
@@ -766,7 +777,7 @@ __global__ __launch_bounds__(256, 2) void pa_bwd_dkv_kernel(const PaArgs a) {
     const int steps = tiles * group, share = __builtin_amdgcn_readfirstlane((steps + a.splits - 1) / a.splits);
     const int begin = split * share < steps ? split * share : steps, end = begin + share < steps ? begin + share : steps;
     const unsigned qo = pa_piece<DHP>(a.q.row, a.dh), po = pa_piece<DHP>(a.dout.row, a.dh);
-    float rst = 0.f;                                                       // threads 0 .. 63: lse of a query, 64 .. 127: its D
+    float rst = 0.f;                                                       // the first ROWS threads: lse of a query, the next: its -D
     // the step that is loaded next: head hd, tile td
     int hd = tiles > 0 ? __builtin_amdgcn_readfirstlane(begin / tiles) : 0, td = begin - hd * tiles;
     auto fetch = [&](int buf) {
@@ -781,7 +792,7 @@ __global__ __launch_bounds__(256, 2) void pa_bwd_dkv_kernel(const PaArgs a) {
                 rst = q < sq.n2 ? a.lse[at] : INFINITY;
                 if (rst == -INFINITY) rst = INFINITY;                      // no key seen, or no query: every probability comes out as zero
             } else
-                rst = q < sq.n2 ? a.dsum[at] : 0.f;
+                rst = q < sq.n2 ? -a.dsum[at] : 0.f;
         }
         if (++td == tiles) { td = 0; ++hd; }
     };
@@ -812,7 +823,14 @@ __global__ __launch_bounds__(256, 2) void pa_bwd_dkv_kernel(const PaArgs a) {
         const float* const lr = s_row + (step & 1) * 2 * ROWS + sub * 32 + h * 4;
         const int q0 = first + q_tile * ROWS + sub * 32;
         if (w_rows > 0 && q0 < sq.n2 && (!a.causal || q0 + 31 + off >= w0)) {
-            f32x16 sc = pa_zero(), dp = pa_zero();
+            f32x16 sc = pa_zero(), dp;                                     // dp: do . v - D, begun with -D
+#pragma unroll
+            for (int g = 0; g < 4; ++g) {
+                const f32x4 dd = *(const f32x4*)(lr + ROWS + g * 8);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) dp[g * 4 + j] = dd[j];
+            }
+            __builtin_amdgcn_sched_group_barrier(0x100, 4, 0);
             __builtin_amdgcn_s_setprio(1);
 #pragma unroll
             for (int kc = 0; kc < KC; ++kc) sc = pa_mfma(pa_row_frag<v8, DHP>(lq + sub * 32 * TL::RB, rp, kc), bk[kc], sc);
@@ -833,8 +851,9 @@ __global__ __launch_bounds__(256, 2) void pa_bwd_dkv_kernel(const PaArgs a) {
             }
             float p[16];
             const int dist0 = ki - (q0 + h * 4 + off), lo = w0 - (q0 + 31 + off), hi = w0 + 31 - (q0 + off);   // distance of the lane's first score; later rows are nearer
-            if (!BIAS || hi <= -a.far || lo >= a.far) {
-                const float b = BIAS ? s_bias[hi <= -a.far ? 0 : 2 * a.far] : 0.f;
+            if (!BIAS) {
+            } else if (hi <= -a.far || lo >= a.far) {
+                const float b = s_bias[hi <= -a.far ? 0 : 2 * a.far];
 #pragma unroll
                 for (int i = 0; i < 16; ++i) p[i] = sc[i] * a.scale2 + b;
             } else if (lo > -a.far && hi < a.far) {
@@ -849,7 +868,7 @@ __global__ __launch_bounds__(256, 2) void pa_bwd_dkv_kernel(const PaArgs a) {
             for (int g = 0; g < 4; ++g) {
                 const f32x4 ls = *(const f32x4*)(lr + g * 8);
 #pragma unroll
-                for (int j = 0; j < 4; ++j) p[g * 4 + j] = __builtin_amdgcn_exp2f(p[g * 4 + j] - ls[j]);
+                for (int j = 0; j < 4; ++j) p[g * 4 + j] = __builtin_amdgcn_exp2f(BIAS ? p[g * 4 + j] - ls[j] : sc[g * 4 + j] * a.scale2 - ls[j]);
             }
             __builtin_amdgcn_s_setprio(1);
 #pragma unroll
@@ -860,11 +879,7 @@ __global__ __launch_bounds__(256, 2) void pa_bwd_dkv_kernel(const PaArgs a) {
             }
             pa_order<2 * MT, 2, 3>();
 #pragma unroll
-            for (int g = 0; g < 4; ++g) {
-                const f32x4 dd = *(const f32x4*)(lr + ROWS + g * 8);
-#pragma unroll
-                for (int j = 0; j < 4; ++j) p[g * 4 + j] *= dp[g * 4 + j] - dd[j];
-            }
+            for (int i = 0; i < 16; ++i) p[i] *= dp[i];
 #pragma unroll
             for (int c = 0; c < 2; ++c) {
                 const v8 r = pa_pack<T>(p + 8 * c);
