@@ -978,9 +978,9 @@ int pa_launch_bwd(PaArgs a, float* dtable, hipStream_t st) {
 // How many workgroups share the queries of 128 keys.  The host knows sizes, not lengths: `groups` of keys, and on average `steps` tiles of
 // queries for each.  Two workgroups fit on a CU, and more than one for each of the 512 places evens them out; but each share is written and
 // read once more in 32 bits, and begins with k, v.  Backward pass in us, one share against the rule's:
-//   336 groups of 74 steps (causal, 128 wide)  532 / 329 (3)      544 of 256 (causal, 128 wide)  1293 / 995 (2)     112 of 44 (causal, 64 wide)  161 / 72 (7)
-//   18 of 16 (64 wide)                          81 / 32 (8)       268 of 128 (64 wide)            447 / 335 (3)
-// and where it leaves one, against two:  512 of 19 (64 wide) 137 / 145,  176 of 8 (causal, 64 wide) 38 / 41,  4288 of 64 (causal, 128 wide) 2100 / 2589.
+//   336 groups of 74 steps (causal, 128 wide)  503 / 317 (3)      544 of 256 (causal, 128 wide)  1220 / 966 (2)     112 of 44 (causal, 64 wide)  138 / 66 (7)
+//   18 of 16 (64 wide)                          73 / 30 (8)       268 of 128 (64 wide)            379 / 307 (3)
+// and where it leaves one, against two:  512 of 19 (64 wide) 118 / 136,  176 of 8 (causal, 64 wide) 33 / 38,  4288 of 64 (causal, 128 wide) 2050 / 2530.
 int pa_splits(const ddpm_packed_attn_desc* d) {
     const long long groups = (long long)(d->Tk / PA_ROWS + d->B + 2) * d->Hk, steps = (long long)d->Tq / PA_TILE * (d->H / d->Hk) / (d->B > 0 ? d->B : 1);
     const long long most = steps / (groups >= 128 ? 16 : 2);               // (half of the card idle: even short shares pay)
