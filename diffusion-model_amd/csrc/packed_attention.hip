@@ -290,6 +290,14 @@ template <typename T> __device__ __forceinline__ typename PaTypes<T>::v8 pa_pack
     return r;
 }
 
+// what rounding to T leaves of it, rounded: a second product with this takes the probabilities to about 2^-16 (bf16), 2^-22 (fp16)
+template <typename T> __device__ __forceinline__ typename PaTypes<T>::v8 pa_rest(const float* s) {
+    typename PaTypes<T>::v8 r;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) r[j] = (T)(s[j] - (float)(T)s[j]);
+    return r;
+}
+
 // ---- relative position bias ----------------------------------------------------------------------------------------------------
 // LDS: the bias of every distance key - query in -far ... far for one head, in units of log2 like the scores.  Finite ones are limited to
 // PA_MAX_BIAS: a row all of whose keys have the same large bias keeps its scores and its normaliser in 32 bits (with a bias of -1e9 both
@@ -434,10 +442,7 @@ __global__ __launch_bounds__(256, 2) void pa_fwd_kernel(const PaArgs a) {
         for (int c = 0; c < 4; ++c) {
             const v8 p = pa_pack<T>(s + 8 * c);
             v8 rest;
-            if constexpr (TWO) {
-#pragma unroll
-                for (int j = 0; j < 8; ++j) rest[j] = (T)(s[8 * c + j] - (float)p[j]);
-            }
+            if constexpr (TWO) rest = pa_rest<T>(s + 8 * c);
 #pragma unroll
             for (int mt = 0; mt < MT; ++mt) {
                 const v8 f = pa_col_frag<v8, DHP>(lv, cp, 16 * c, mt);
@@ -528,6 +533,10 @@ __global__ __launch_bounds__(256, 2) void pa_bwd_dq_kernel(const PaArgs a) {
     keys = keys < 0 ? 0 : keys < sq.n2 ? keys : sq.n2;
     const int tiles = (keys + PA_TILE - 1) / PA_TILE;
     const bool sweep = tiles <= 2;
+    // ds in two parts where its rounding shows: few keys, whose terms do not average out, and narrow heads, whose weighted mean of the keys
+    // is not small against the keys and cancels (the sum of a row's ds is zero).  dq's error, in multiples of one rounding of the result: 1.4 to 2.6
+    // with one part and few keys, 1.6 with heads of 8; 1.0 with two.  (The branch costs long rows of wide heads 2 %.)
+    const bool two = sweep || DHP == 32;
     const float lse = qv ? a.lse[(long long)head * a.Tq + row] : 0.f;
     float dsum = 0.f;
     if (sweep) {
@@ -687,6 +696,14 @@ __global__ __launch_bounds__(256, 2) void pa_bwd_dq_kernel(const PaArgs a) {
                 }
                 pa_order<2 * MT, 2, 3>();
                 __builtin_amdgcn_s_setprio(0);
+                if (two) {
+#pragma unroll
+                    for (int c = 0; c < 2; ++c) {
+                        const v8 r = pa_rest<T>(ds + 8 * c);
+#pragma unroll
+                        for (int mt = 0; mt < MT; ++mt) acc[mt] = pa_mfma(pa_col_frag<v8, DHP>(lk, cp, sub * 32 + 16 * c, mt), r, acc[mt]);
+                    }
+                }
             }
         }
     }
@@ -774,6 +791,7 @@ __global__ __launch_bounds__(256, 2) void pa_bwd_dkv_kernel(const PaArgs a) {
     int first = a.causal ? sq.row0 - off : 0;                              // the first query that sees any key of the workgroup
     first = first < 0 ? 0 : first / ROWS * ROWS;
     const int tiles = sq.n2 > first ? (sq.n2 - first + ROWS - 1) / ROWS : 0;
+    const bool two = sq.n2 <= 2 * PA_TILE || DHP == 32;                    // p and ds in two parts: few queries, narrow heads (see the pass over queries)
     const int steps = tiles * group, share = __builtin_amdgcn_readfirstlane((steps + a.splits - 1) / a.splits);
     const int begin = split * share < steps ? split * share : steps, end = begin + share < steps ? begin + share : steps;
     const unsigned qo = pa_piece<DHP>(a.q.row, a.dh), po = pa_piece<DHP>(a.dout.row, a.dh);
@@ -878,6 +896,14 @@ __global__ __launch_bounds__(256, 2) void pa_bwd_dkv_kernel(const PaArgs a) {
                 for (int mt = 0; mt < MT; ++mt) dv[mt] = pa_mfma(pa_col_frag<v8, DHP>(lp, cp, sub * 32 + 16 * c, mt), r, dv[mt]);
             }
             pa_order<2 * MT, 2, 3>();
+            if (two) {
+#pragma unroll
+                for (int c = 0; c < 2; ++c) {
+                    const v8 r = pa_rest<T>(p + 8 * c);
+#pragma unroll
+                    for (int mt = 0; mt < MT; ++mt) dv[mt] = pa_mfma(pa_col_frag<v8, DHP>(lp, cp, sub * 32 + 16 * c, mt), r, dv[mt]);
+                }
+            }
 #pragma unroll
             for (int i = 0; i < 16; ++i) p[i] *= dp[i];
 #pragma unroll
@@ -888,6 +914,14 @@ __global__ __launch_bounds__(256, 2) void pa_bwd_dkv_kernel(const PaArgs a) {
             }
             pa_order<2 * MT, 2, 3>();
             __builtin_amdgcn_s_setprio(0);
+            if (two) {
+#pragma unroll
+                for (int c = 0; c < 2; ++c) {
+                    const v8 r = pa_rest<T>(p + 8 * c);
+#pragma unroll
+                    for (int mt = 0; mt < MT; ++mt) dk[mt] = pa_mfma(pa_col_frag<v8, DHP>(lq, cp, sub * 32 + 16 * c, mt), r, dk[mt]);
+                }
+            }
         }
         }
         if (++q_tile == tiles) { q_tile = 0; ++q_head; }

@@ -119,9 +119,9 @@ class _PackedAttentionFn(torch.autograd.Function):
     def forward(ctx, q, k, v, table, ends_q, ends_k, bucket_of, causal: bool, scale: Optional[float]):
         _note_graph(ctx, q, k, v, table)
         q, k, v = _heads(q), _heads(k), _heads(v)
-        train = any(ctx.needs_input_grad)
+        train = any(ctx.needs_input_grad)                 # (narrow heads: the rounding of o would show in dq)
         o, lse, o32 = ops.packed_attention_forward(q, k, v, ends_q, ends_k, causal=causal, scale=scale, table=table, bucket_of=bucket_of,
-                                                   want_lse=train, want_o32=table is not None and ctx.needs_input_grad[3])
+                                                   want_lse=train, want_o32=train and (q.shape[2] <= 32 or (table is not None and ctx.needs_input_grad[3])))
         ctx.save_for_backward(q, k, v, table, ends_q, ends_k, bucket_of, o, lse, o32)
         ctx.how = (causal, scale)
         return o
@@ -132,7 +132,7 @@ class _PackedAttentionFn(torch.autograd.Function):
         _refuse_stale(ctx, "packed_attention")
         q, k, v, table, ends_q, ends_k, bucket_of, o, lse, o32 = ctx.saved_tensors
         dq, dk, dv, dtable = ops.packed_attention_backward(q, k, v, o, lse, _heads(dout), ends_q, ends_k, causal=ctx.how[0], scale=ctx.how[1], table=table,
-                                                           bucket_of=bucket_of, o32=o32, want_dtable=o32 is not None)
+                                                           bucket_of=bucket_of, o32=o32, want_dtable=ctx.needs_input_grad[3])
         return dq, dk, dv, dtable, None, None, None, None, None
 
 
