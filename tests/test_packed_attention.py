@@ -338,6 +338,27 @@ def test_captured_and_on_another_stream(dev):
 
 
 @pytest.mark.gpu
+def test_capture_beside_a_living_graph_is_refused(dev):
+    d = make([9, 20], [9, 20], 2, 1, 32, torch.bfloat16, seed=20, table=(8, 6, True))
+    q, k, v, ends, do = (d[n].to(dev) for n in ("q", "k", "v", "eq", "do"))
+    table, how = d["table"].to(dev).requires_grad_(), dict(bias_buckets=d["buckets"].to(dev))
+    old = sequence.packed_attention(q, k, v, ends, bias_table=table, **how)
+    with pytest.raises(RuntimeError, match="packed_attention.*is alive"):
+        with torch.cuda.graph(torch.cuda.CUDAGraph()):
+            torch.autograd.grad(sequence.packed_attention(q, k, v, ends, bias_table=table, **how), table, do)
+    torch.cuda.synchronize()
+    want, = torch.autograd.grad(old, table, do)
+    del old
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        got, = torch.autograd.grad(sequence.packed_attention(q, k, v, ends, bias_table=table, **how), table, do)
+    for _ in range(2):
+        g.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(got, want)
+
+
+@pytest.mark.gpu
 def test_many_sequences(dev):
     """more sequences than a wave has lanes, most of them shorter than a tile"""
     g = torch.Generator().manual_seed(15)
