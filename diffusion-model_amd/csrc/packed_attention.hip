@@ -242,6 +242,14 @@ template <typename V8, int DHP> __device__ __forceinline__ V8 pa_col_frag(const 
     const s16x8 r = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
     return __builtin_bit_cast(V8, r);
 }
+// ds as a 32-bit number: in fp16 the compiler would take the 16-bit part straight from the product of its factors (one rounding, v_fma_mix) and the rest
+// from the product in 32 bits (two), which differ by a whole step once in some thousand pairs
+template <typename T> __device__ __forceinline__ void pa_settle(float (&ds)[16]) {
+    if constexpr (std::is_same<T, f16>::value) {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) asm volatile("" : "+v"(ds[i]));
+    }
+}
 template <int DHP> __device__ __forceinline__ void pa_opaque(unsigned& place) {
     if constexpr (DHP == 128) asm volatile("" : "+v"(place));
 }
@@ -655,6 +663,7 @@ __global__ __launch_bounds__(256, 2) void pa_bwd_dq_kernel(const PaArgs a) {
                     ds[i] = p[i] * dp[i];
                     sum += ds[i];
                 }
+                pa_settle<T>(ds);
                 all += sum;
                 if (want_table) {
                     const int lo = k0 - (w0 + 31 + off), hi = k0 + 31 - (w0 + off);
@@ -906,6 +915,7 @@ __global__ __launch_bounds__(256, 2) void pa_bwd_dkv_kernel(const PaArgs a) {
             }
 #pragma unroll
             for (int i = 0; i < 16; ++i) p[i] *= dp[i];
+            pa_settle<T>(p);
 #pragma unroll
             for (int c = 0; c < 2; ++c) {
                 const v8 r = pa_pack<T>(p + 8 * c);

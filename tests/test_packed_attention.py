@@ -9,6 +9,8 @@ Tolerances, per element, from worst cases of every rounding (u = half a step of 
   own rounding u |ds| (+ 2^-25 in fp16); dq, dk, dv: those errors times |k|, |q|, |do|, summed, plus n 2^-24 of the terms, plus u of the result.
   A result in fp16 below 2^-14 is a multiple of 2^-24: its rounding is 2^-25 then, not u of it (dv = -1.1177008771e-05 of one case is
   2.87e-08 from the nearest fp16 number, by the format alone).
+  Rows of at most 128 keys, keys of at most 128 queries (two=True): p and ds of the backward products in two parts, u^2 in place of u (what the first
+  part leaves is exact in 32 bits), twice the terms to sum, and D as the sum of p (do.v), each with its own errors above and n 2^-24.
   dtable: the 32-bit ds, D from an output whose p had an error of u^2 instead of u; a sum of all pairs of a bucket, m 2^-24 at most for the
   m terms of one row of tiles (64 of them per step, then steps, waves and slots in turn: 2^-24 (64 + 512) used)."""
 import ctypes
@@ -37,7 +39,7 @@ def make(lens_q, lens_k, heads, kv, width, dtype, seed=0, tail=0, lead=0, table=
     return d
 
 
-def reference(d, causal, scale=None):
+def reference(d, causal, scale=None, two=False):
     """results and tolerances in float64, sequence by sequence"""
     dtype, heads, kv, width = d["q"].dtype, d["q"].shape[1], d["k"].shape[1], d["q"].shape[2]
     u, floor = HALF_STEP[dtype], (2.0 ** -25 if dtype == torch.float16 else 0.0)
@@ -82,6 +84,10 @@ def reference(d, causal, scale=None):
         eds32 = ds.abs() * ep + p * (err_dp + err_d((u * u + base) * terms + miss * u + 2.0 ** -23 * o.abs()))
         eds = ds.abs() * (ep + u) + p * (err_dp + err_d(to + u * o.abs())) + floor * seen
         ep16 = p * (u + ep) + floor * seen
+        if two:
+            e_d = (p * (dp.abs() * (ep + nk * 2.0 ** -24) + err_dp)).sum(-1, keepdim=True)
+            eds = ds.abs() * (ep + u * u + (nk + nq * heads // kv) * 2.0 ** -24) + p * (err_dp + e_d) + floor * seen
+            ep16 = p * (u * u + ep + nq * heads // kv * 2.0 ** -24) + floor * seen
         add = lambda name, rows, x, t: (out[name][rows].add_(x), tol[name][rows].add_(t))  # noqa: E731
         add("o", rq, o.permute(1, 0, 2), (to + u * o.abs() + floor).permute(1, 0, 2))
         add("dq", rq, (scale * ds @ K).permute(1, 0, 2), (scale * ((eds + nk * 2.0 ** -24 * ds.abs()) @ K.abs()) + u * (scale * ds @ K).abs() + floor).permute(1, 0, 2))
@@ -130,6 +136,18 @@ LENS = {"one": [1], "short": [3, 1, 0, 17, 2], "tiles": [64, 32, 128, 31, 33, 63
 def test_against_float64(dev, dtype, causal, lens, heads, kv, width):
     d = make(LENS[lens], LENS[lens], heads, kv, width, dtype, seed=width, tail=5)
     compare(d, dev, causal, cross=False)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("causal", [False, True])
+@pytest.mark.parametrize("heads,kv,width", [(2, 2, 64), (4, 1, 128), (2, 1, 8), (3, 3, 40)])
+def test_gradients_of_short_sequences_have_one_rounding(dev, dtype, causal, heads, kv, width):
+    d = make([2, 1, 5, 17, 64, 100, 128, 3], [2, 1, 5, 17, 64, 100, 128, 3], heads, kv, width, dtype, seed=19)
+    got = run(d, dev, causal)
+    want, tol = reference(d, causal, two=True)
+    for n in ("dq", "dk", "dv"):
+        check(n, got[n], want[n], tol[n])
 
 
 @pytest.mark.gpu
