@@ -545,7 +545,9 @@ __global__ __launch_bounds__(256, 2) void pa_bwd_dq_kernel(const PaArgs a) {
     // is not small against the keys and cancels (the sum of a row's ds is zero).  dq's error, in multiples of one rounding of the result: 1.4 to 2.6
     // with one part and few keys, 1.6 with heads of 8; 1.0 with two.  (The branch costs long rows of wide heads 2 %.)
     const bool two = sweep || DHP == 32;
-    const float lse = qv ? a.lse[(long long)head * a.Tq + row] : 0.f;
+    // (-inf: no key seen, as where a bias of -inf hides all of them.  As +inf, every probability comes out as zero; -inf - -inf would be NaN)
+    float lse = qv ? a.lse[(long long)head * a.Tq + row] : 0.f;
+    if (lse == -INFINITY) lse = INFINITY;
     float dsum = 0.f;
     if (sweep) {
     } else if (a.o32) {
