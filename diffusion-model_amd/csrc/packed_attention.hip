@@ -250,6 +250,34 @@ template <typename T> __device__ __forceinline__ void pa_settle(float (&ds)[16])
         for (int i = 0; i < 16; ++i) asm volatile("" : "+v"(ds[i]));
     }
 }
+// Operands in fp16 lie within its normal numbers, 2^-14 to 65504, or lose bits; probabilities and ds of long rows do not: about 1 / keys, and that times
+// the output gradient.  So p carries a factor of 2^12 in the pass over keys (it is at most 1), and ds a power of two per owned row, i.e. per lane:
+// `up` brings the row's largest ds so far between 2^8 and 2^15, falls when a larger one comes, the row's accumulators with it, and is taken out
+// of the result.  Powers of two round nothing.  bf16 has the exponents of 32 bits and takes neither.  Without it dq's error is 6.9 times what the
+// roundings explain with output gradients of 1e-3, 4096 keys and heads of 64 (ds down to 2^-24 steps); it costs the fp16 backward pass 4 to 11 % (batch of
+// 2048 ... 1 causal tokens, 16 heads of 128 over 4: 330 -> 343 us), 13 % with heads of 32.
+template <typename T> struct PaRange { static constexpr float P_LOG = 0.f, P_OFF = 1.f, UP = 1.f; };
+template <> struct PaRange<f16> { static constexpr float P_LOG = 12.f, P_OFF = 0x1p-12f, UP = 0x1p60f; };
+template <typename T, int MT> __device__ __forceinline__ void pa_raise(float (&ds)[16], float& up, f32x16 (&acc)[MT]) {
+    if constexpr (std::is_same<T, f16>::value) {
+        float top = 0.f;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) top = fmaxf(top, fabsf(ds[i]));
+        top = pa_half_max(top);
+        if (__any(top * up > 0x1p15f)) {
+            // 2^8 / the power of two in top (its exponent is at least -45 here, at most 128 for infinity)
+            const unsigned to = top * up > 0x1p15f ? (262u - (__float_as_uint(top) >> 23)) << 23 : __float_as_uint(up);
+            const float by = __builtin_amdgcn_ldexpf(1.f, (int)(to >> 23) - (int)(__float_as_uint(up) >> 23));
+            up = __uint_as_float(to);
+#pragma unroll
+            for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) acc[mt][i] *= by;
+        }
+#pragma unroll
+        for (int i = 0; i < 16; ++i) ds[i] *= up;
+    }
+}
 template <int DHP> __device__ __forceinline__ void pa_opaque(unsigned& place) {
     if constexpr (DHP == 128) asm volatile("" : "+v"(place));
 }
@@ -531,6 +559,7 @@ __global__ __launch_bounds__(256, 2) void pa_bwd_dq_kernel(const PaArgs a) {
     const int on_tile = lane <= 31 ? (2 << lane) - 1 : lane < 63 ? -1 << (lane - 31) : 0;
     float before = 0.f, after = 0.f, pbefore = 0.f, pafter = 0.f;          // ds and p at distances <= -far, >= far
     float all = 0.f;                                                       // every ds of the row
+    float up = PaRange<T>::UP;
 
     const int w_rows = sq.n - w0 < 32 ? sq.n - w0 : 32;
     v8 bq[KC], bdo[KC];
@@ -698,6 +727,7 @@ __global__ __launch_bounds__(256, 2) void pa_bwd_dq_kernel(const PaArgs a) {
                     }
                 }
                 // ds is rounded to the type of k for the product (see p in the forward pass)
+                pa_raise<T, MT>(ds, up, acc);
                 __builtin_amdgcn_s_setprio(1);
 #pragma unroll
                 for (int c = 0; c < 2; ++c) {
@@ -720,7 +750,8 @@ __global__ __launch_bounds__(256, 2) void pa_bwd_dq_kernel(const PaArgs a) {
     }
     all = pa_half_sum(all);
     if (qv && h == 0) a.dsum[(long long)head * a.Tq + row] = dsum + all;
-    pa_put<T, DHP>(acc, pa_rows(a.dq, sq.begin + w0, w_rows, head, a.dh), [&](float x) { return x * a.scale; });
+    const float out = a.scale / up;
+    pa_put<T, DHP>(acc, pa_rows(a.dq, sq.begin + w0, w_rows, head, a.dh), [&](float x) { return x * out; });
     if (!want_table) return;
     before = wave_sum(before - all * pbefore);
     after = wave_sum(after - all * pafter);
@@ -806,6 +837,7 @@ __global__ __launch_bounds__(256, 2) void pa_bwd_dkv_kernel(const PaArgs a) {
     const int steps = tiles * group, share = __builtin_amdgcn_readfirstlane((steps + a.splits - 1) / a.splits);
     const int begin = split * share < steps ? split * share : steps, end = begin + share < steps ? begin + share : steps;
     const unsigned qo = pa_piece<DHP>(a.q.row, a.dh), po = pa_piece<DHP>(a.dout.row, a.dh);
+    float up = PaRange<T>::UP;
     float rst = 0.f;                                                       // the first ROWS threads: lse of a query, the next: its -D
     // the step that is loaded next: head hd, tile td
     int hd = tiles > 0 ? __builtin_amdgcn_readfirstlane(begin / tiles) : 0, td = begin - hd * tiles;
@@ -818,7 +850,7 @@ __global__ __launch_bounds__(256, 2) void pa_bwd_dkv_kernel(const PaArgs a) {
             const int q = q0 + (threadIdx.x & (ROWS - 1));
             const long long at = (long long)head * a.Tq + sq.begin2 + q;
             if (threadIdx.x < ROWS) {
-                rst = q < sq.n2 ? a.lse[at] : INFINITY;
+                rst = q < sq.n2 ? a.lse[at] - PaRange<T>::P_LOG : INFINITY;
                 if (rst == -INFINITY) rst = INFINITY;                      // no key seen, or no query: every probability comes out as zero
             } else
                 rst = q < sq.n2 ? -a.dsum[at] : 0.f;
@@ -918,6 +950,7 @@ __global__ __launch_bounds__(256, 2) void pa_bwd_dkv_kernel(const PaArgs a) {
 #pragma unroll
             for (int i = 0; i < 16; ++i) p[i] *= dp[i];
             pa_settle<T>(p);
+            pa_raise<T, MT>(p, up, dk);
 #pragma unroll
             for (int c = 0; c < 2; ++c) {
                 const v8 r = pa_pack<T>(p + 8 * c);
@@ -939,6 +972,7 @@ __global__ __launch_bounds__(256, 2) void pa_bwd_dkv_kernel(const PaArgs a) {
         if (++q_tile == tiles) { q_tile = 0; ++q_head; }
         if (step + 1 < end) keep((step + 1) & 1);
     }
+    const float k_out = PaRange<T>::P_OFF / up;
     if (a.dkv_part) {
         if (!kv) return;
         const long long row = sq.begin + ki;
@@ -949,14 +983,14 @@ __global__ __launch_bounds__(256, 2) void pa_bwd_dkv_kernel(const PaArgs a) {
             for (int g = 0; g < 4; ++g) {
                 const int d = mt * 32 + g * 8 + h * 4;
                 if (d < a.dh) {
-                    *(f32x4*)(p + d) = f32x4{dk[mt][g * 4], dk[mt][g * 4 + 1], dk[mt][g * 4 + 2], dk[mt][g * 4 + 3]};
-                    *(f32x4*)(p2 + d) = f32x4{dv[mt][g * 4], dv[mt][g * 4 + 1], dv[mt][g * 4 + 2], dv[mt][g * 4 + 3]};
+                    *(f32x4*)(p + d) = f32x4{dk[mt][g * 4], dk[mt][g * 4 + 1], dk[mt][g * 4 + 2], dk[mt][g * 4 + 3]} * k_out;
+                    *(f32x4*)(p2 + d) = f32x4{dv[mt][g * 4], dv[mt][g * 4 + 1], dv[mt][g * 4 + 2], dv[mt][g * 4 + 3]} * PaRange<T>::P_OFF;
                 }
             }
         return;
     }
-    pa_put<T, DHP>(dk, pa_rows(a.dk, sq.begin + w0, w_rows, hk, a.dh), [&](float x) { return x * a.scale; });
-    pa_put<T, DHP>(dv, pa_rows(a.dv, sq.begin + w0, w_rows, hk, a.dh), [&](float x) { return x; });
+    pa_put<T, DHP>(dk, pa_rows(a.dk, sq.begin + w0, w_rows, hk, a.dh), [&](float x) { return x * (a.scale * k_out); });
+    pa_put<T, DHP>(dv, pa_rows(a.dv, sq.begin + w0, w_rows, hk, a.dh), [&](float x) { return x * PaRange<T>::P_OFF; });
 }
 
 // dk, dv = the sums over the splits, in order: a thread takes four elements of a row of both
