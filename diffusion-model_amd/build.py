@@ -2,8 +2,8 @@
 
     python diffusion-model_amd/build.py [--force] [-j N]
 
-Each translation unit is compiled to build/<name>.o (skipped when up to date) and the objects are
-linked into lib/libddpm_hip.so.  Nothing but hipcc and the HIP runtime is needed: the library has a
+Each translation unit is compiled to build/<name>.o (skipped when it is newer than its sources and was made by the
+same command, which build/<name>.o.cmd holds) and the objects are linked into lib/libddpm_hip.so.  Nothing but hipcc and the HIP runtime is needed: the library has a
 plain C ABI (include/ddpm_hip.h) and no dependency on torch.
 """
 from __future__ import annotations
@@ -32,6 +32,19 @@ def _stale(target: str, deps) -> bool:
     return any(os.path.getmtime(d) > t for d in deps)
 
 
+def _command(source: str, target: str):
+    return [HIPCC] + FLAGS + ["-c", source, "-o", target]
+
+
+def _made_by(target: str) -> str:
+    """The command that made this object (empty: not known, or its last compilation failed)"""
+    try:
+        with open(target + ".cmd") as f:
+            return f.read()
+    except OSError:
+        return ""
+
+
 def build(force: bool = False, jobs: int = 8, verbose: bool = True) -> str:
     os.makedirs(OBJ, exist_ok=True)
     os.makedirs(LIBDIR, exist_ok=True)
@@ -42,13 +55,18 @@ def build(force: bool = False, jobs: int = 8, verbose: bool = True) -> str:
     for s in sources:
         o = os.path.join(OBJ, os.path.basename(s)[:-4] + ".o")
         objs.append(o)
-        if force or _stale(o, [s] + headers):
+        if force or _stale(o, [s] + headers) or _made_by(o) != " ".join(_command(s, o)):
             todo.append((s, o))
 
     def cc(pair):
         s, o = pair
-        cmd = [HIPCC] + FLAGS + ["-c", s, "-o", o]
+        cmd = _command(s, o)
+        if os.path.exists(o + ".cmd"):
+            os.remove(o + ".cmd")
         r = subprocess.run(cmd, capture_output=True, text=True)
+        if r.returncode == 0:
+            with open(o + ".cmd", "w") as f:
+                f.write(" ".join(cmd))
         lines = (r.stdout + r.stderr).splitlines()
         return s, r.returncode, "\n".join(ln for ln in lines if "'-packed-fp32-ops' is not a recognized feature" not in ln)
 
