@@ -10,6 +10,7 @@ from typing import Optional
 
 import torch
 from torch import Tensor, nn
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from ..runtime import hip, ops
@@ -22,6 +23,12 @@ def _need_gpu(what: str, *tensors) -> None:
     for t in tensors[1:]:
         if t is not None and t.device != dev:
             raise ValueError(f"{what}: tensors on {dev} and {t.device}")
+
+
+def _no_tangents(what: str, *tensors) -> None:
+    """A dual tensor need not ask for a gradient: past the autograd function its tangent would be lost without a word"""
+    if forward_ad._current_level >= 0 and any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+        raise NotImplementedError(f"{what}: forward-mode derivatives (jvp) are not there")
 
 
 def _wants_grad(*tensors) -> bool:
@@ -81,9 +88,10 @@ class _LayerNormFn(torch.autograd.Function):
 
 def layer_norm(x: Tensor, weight: Optional[Tensor] = None, bias: Optional[Tensor] = None, eps: float = 1e-5) -> Tensor:
     """(x - mean) / sqrt(var + eps) * weight + bias over the last axis (1 to 8192 elements, var over n), statistics in fp32, the
-    result in x's type.  weight, bias: fp32 [C] or None.  Differentiable once in x, weight and bias."""
+    result in x's type.  weight, bias: fp32 [C] or None.  Differentiable once in x, weight and bias (in reverse mode)."""
     if x.dim() < 1 or x.shape[-1] < 1:
         raise ValueError(f"layer_norm: x of shape {tuple(x.shape)} has no last axis to normalise")
+    _no_tangents("layer_norm", x, weight, bias)
     _need_gpu("layer_norm", x, weight, bias)
     if not _wants_grad(x, weight, bias):                  # (a graph node costs a third of a short call's host time)
         return ops.layer_norm_forward(_rows(x, x.shape[-1]), weight, bias, float(eps), want_stats=False)[0].view(x.shape)
@@ -150,10 +158,11 @@ def packed_attention(q: Tensor, k: Tensor, v: Tensor, ends: Tensor, *, ends_k: O
     bias_table [buckets, heads] (fp32, learned) with bias_buckets [2 far + 1] (int32, relative_position_buckets): adds
     bias_table[bucket of (key's place - query's place), head] to the score.  A bias of -inf hides its distances; finite ones beyond +-5678
     (2^13 powers of two) count as that.
-    Differentiable once in q, k, v and bias_table."""
+    Differentiable once in q, k, v and bias_table (in reverse mode)."""
     for name, t in (("q", q), ("k", k), ("v", v)):
         if t.dim() != 3:
             raise ValueError(f"packed_attention: {name} of shape {tuple(t.shape)} is not [tokens, heads, width]")
+    _no_tangents("packed_attention", q, k, v, bias_table)
     _need_gpu("packed_attention", q, k, v, ends, ends_k, bias_table, bias_buckets)
     if not _wants_grad(q, k, v, bias_table):
         return ops.packed_attention_forward(_heads(q), _heads(k), _heads(v), ends, ends_k, causal=bool(causal), scale=scale, table=bias_table,
