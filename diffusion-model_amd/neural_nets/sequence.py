@@ -5,6 +5,7 @@ everywhere in this package.  The reference has no such encoder; its ConditionalM
 (constituent_blocks.py:402-437 there)."""
 from __future__ import annotations
 
+import threading
 import weakref
 from typing import Optional
 
@@ -44,6 +45,7 @@ def _rows(t: Tensor, c: int) -> Tensor:
 
 
 _graphs: list = []                   # weak references to the nodes of this module's autograd graphs, dead ones swept now and then
+_graphs_lock = threading.RLock()     # (held by sweeps and notes: a node noted between a sweep's look and its end would be lost)
 
 
 def _note_graph(ctx, *inputs) -> None:
@@ -52,12 +54,15 @@ def _note_graph(ctx, *inputs) -> None:
     the backward pass of a captured graph looks for such a graph, and refuses in time."""
     ctx.stream, ctx.stale = hip.stream(), False
     if ctx.stream == 0:
-        _graphs.append(weakref.ref(ctx))
-        if len(_graphs) >= 4096:
-            _graphs[:] = [r for r in _graphs if r() is not None]
+        with _graphs_lock:
+            _graphs.append(weakref.ref(ctx))
+            if len(_graphs) >= 4096:
+                _graphs[:] = [r for r in _graphs if r() is not None]
     elif torch.cuda.is_current_stream_capturing():
         leaves = [t for t in inputs if t is not None and t.requires_grad and t.is_leaf]
-        held = [getattr(node, "variable", None) for r in _graphs if (graph := r()) is not None for node, _ in graph.next_functions]
+        with _graphs_lock:
+            noted = list(_graphs)
+        held = [getattr(node, "variable", None) for r in noted if (graph := r()) is not None for node, _ in graph.next_functions]
         ctx.stale = any(h is t for h in held if h is not None for t in leaves)
 
 

@@ -1,0 +1,33 @@
+"""The list of living autograd graphs, by which a captured backward pass is refused in time, with several threads at work on it."""
+import threading
+
+import torch
+
+from dm_amd.neural_nets import sequence
+from dm_amd.runtime import hip
+
+
+class Node:
+    next_functions = ()
+
+
+def test_a_graph_noted_during_a_sweep_is_kept(monkeypatch):
+    """one thread sweeps dead entries out; another notes a graph just before the swept list is put in place"""
+    monkeypatch.setattr(hip, "stream", lambda *a: 0)
+    late, threads = Node(), []
+
+    class Slow(list):
+        def __setitem__(self, at, value):
+            t = threading.Thread(target=sequence._note_graph, args=(late, torch.zeros(1)))
+            threads.append(t)
+            t.start()
+            t.join(0.3)                                        # (it either gets through, or waits for the sweep to end)
+            super().__setitem__(at, value)
+
+    graphs = Slow([lambda: None] * 4095)
+    monkeypatch.setattr(sequence, "_graphs", graphs)
+    first = Node()
+    sequence._note_graph(first, torch.zeros(1))
+    assert len(threads) == 1
+    threads[0].join(10)
+    assert not threads[0].is_alive() and {r() for r in graphs} == {first, late}
