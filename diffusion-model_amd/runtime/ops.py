@@ -695,6 +695,8 @@ def grad_norm(grads, norm_type: float = 2.0, max_norm: Optional[float] = None) -
     at, n, size = _merge_spans(at, n, size)
     norm = torch.empty((), device=dev, dtype=torch.float32)
     launch_grad_norm(at, n, size, kinds[float(norm_type)], max_norm, norm)
+    if max_norm is not None:
+        torch.autograd.graph.increment_version(grads)      # (written by address: autograd has to be told)
     return norm
 
 
