@@ -29,7 +29,8 @@ class FusedAdam(torch.optim.Optimizer):
     max_grad_norm: clip the gradients' global 2-norm (times grad_scale, if step() is given one) to this value, as
     clip_grad_norm_(parameters, max_grad_norm) before the step would; the update reads the norm and scales the gradients on the way,
     so .grad keeps its values and no pass writes clipped ones.  `grad_norm` holds the last step's norm before clipping (a 0-dim
-    tensor on the device).  The norm needs every gradient: step_ranges() refuses.
+    tensor on the device).  The norm needs every gradient: step_ranges() refuses.  A captured step() keeps the limit it was captured with; the
+    graph drivers refuse to replay one after max_grad_norm has changed.
 
     One hyper-parameter set for all parameters: several param groups are accepted only when their lr, betas, eps and
     weight_decay agree."""

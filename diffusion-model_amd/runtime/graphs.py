@@ -37,6 +37,17 @@ def _pool_stream(device, k: int = 0) -> "torch.cuda.Stream":
     return pool[k]
 
 
+def _limit(optimizer):
+    return getattr(optimizer, "max_grad_norm", None)
+
+
+def _same_limit(optimizer, captured) -> None:
+    """The limit of an optimizer that clips travels in the captured launches: another one would have no effect, and say nothing"""
+    if _limit(optimizer) != captured:
+        raise RuntimeError(f"the optimizer's max_grad_norm is {_limit(optimizer)}, but this step was captured with {captured}: build the step again to capture "
+                           "the new limit")
+
+
 class GraphedTrainStep:
     """randint t -> q -> UNet -> ELBO -> backward -> [grad hook, e.g. all-reduce] -> optimizer.step, as one graph.
 
@@ -80,6 +91,7 @@ class GraphedTrainStep:
                 self.graph2 = torch.cuda.CUDAGraph()
                 with torch.cuda.graph(self.graph2, capture_error_mode="thread_local"):
                     self._back()
+            self._captured_limit = _limit(optimizer)
 
     def _front(self):
         n = self.x0.shape[0]
@@ -106,6 +118,8 @@ class GraphedTrainStep:
         self._back()
 
     def replay(self) -> Tensor:
+        if self.graph is not None:
+            _same_limit(self.optimizer, self._captured_limit)
         if hasattr(self.optimizer, "sync_lr"):
             self.optimizer.sync_lr()            # an LR scheduler's new value reaches the captured Adam through device memory
         if self.graph is None:
@@ -252,6 +266,7 @@ class PipelinedTrainStep:
                     self._adam()
             torch.cuda.synchronize()
             self.graphs = (gm, gw, gc, gp)
+            self._captured_limit = _limit(optimizer)
 
     # ---- pieces ------------------------------------------------------------------------------------------------------
     @torch.no_grad()
@@ -469,6 +484,8 @@ class PipelinedTrainStep:
 
     def replay(self, last: bool = False) -> Tensor:
         """One micro-step on the batch in self.x0; last=True forces the optimizer step (the trainer's last batch of an epoch)."""
+        if self.graphs is not None:
+            _same_limit(self.optimizer, self._captured_limit)
         if hasattr(self.optimizer, "sync_lr"):
             self.optimizer.sync_lr()            # an LR scheduler's new value reaches the captured Adam through device memory
         self._run(self.graphs, last=last)
