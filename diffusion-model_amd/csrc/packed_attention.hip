@@ -1134,7 +1134,9 @@ int pa_setup(const ddpm_packed_attn_desc* d, bool bwd, PaArgs& a) {
 
 extern "C" int ddpm_packed_attn_slots(int Tq, int B) { return Tq / PA_ROWS + B + 2; }
 extern "C" int64_t ddpm_packed_attn_dkv_floats(const ddpm_packed_attn_desc* d) {
-    const int splits = d && d->Hk > 0 ? pa_splits(d) : 1;
+    // (sizes that the backward pass refuses need nothing)
+    const bool sizes = d && d->H > 0 && d->Hk > 0 && d->Tq >= 0 && d->Tk >= 0 && d->B >= 0 && d->Tq < (1 << 30) && d->Tk < (1 << 30) && d->B < (1 << 24);
+    const int splits = sizes ? pa_splits(d) : 1;
     return splits > 1 ? 2ll * splits * d->Tk * d->Hk * d->dh : 0;
 }
 
