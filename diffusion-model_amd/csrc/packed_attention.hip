@@ -343,8 +343,8 @@ __device__ __forceinline__ void pa_bias_fill(const PaArgs& a, int head, float* s
     for (int i = threadIdx.x; i < 2 * a.far + 1; i += blockDim.x) {
         int b = a.bucket_of[i];
         b = b < 0 ? 0 : b >= a.buckets ? a.buckets - 1 : b;
-        const float x = a.table[b * a.H + head] * 1.4426950408889634f;
-        s_bias[i] = fabsf(a.table[b * a.H + head]) < INFINITY ? fminf(fmaxf(x, -PA_MAX_BIAS), PA_MAX_BIAS) : x;
+        const float t = a.table[(long long)b * a.H + head], x = t * 1.4426950408889634f;
+        s_bias[i] = fabsf(t) < INFINITY ? fminf(fmaxf(x, -PA_MAX_BIAS), PA_MAX_BIAS) : x;
     }
 }
 __device__ __forceinline__ int pa_clamp(int d, int far) { return d < -far ? -far : d > far ? far : d; }

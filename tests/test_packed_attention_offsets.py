@@ -1,0 +1,45 @@
+"""Packed attention with offsets past 32 bits and neighbours in memory that must not arrive."""
+import pytest
+import torch
+
+from dm_amd.neural_nets import sequence
+
+
+@pytest.mark.gpu
+def test_a_bias_table_of_more_than_two_to_the_31_elements(dev):
+    """two tokens, 32800 heads, 65536 buckets, the last two of them used: o is the mean of two values with weights 1 / (1 + exp(s1 - s0)).  Bound: p rounded
+    to bf16 and the result's rounding, 2^-8 each, of sums of |v|."""
+    heads, buckets = 32800, 65536
+    assert (buckets - 2) * heads > 2 ** 31
+    g = torch.Generator(dev).manual_seed(1)
+    q, k, v = (torch.randn(2, heads, 8, generator=g, device=dev).bfloat16() for _ in range(3))
+    table = torch.zeros(buckets, heads, device=dev)
+    table[-2:] = torch.randn(2, heads, generator=g, device=dev) * 3
+    which = torch.full((9,), buckets - 2, dtype=torch.int32, device=dev)
+    which[4] = buckets - 1                                     # the own place
+    o = sequence.packed_attention(q, k, v, torch.tensor([0, 2], dtype=torch.int32, device=dev), bias_table=table, bias_buckets=which)
+    s = (q.double()[:, None] * k.double()[None]).sum(-1) * 8 ** -0.5          # [query, key, head]
+    s += torch.stack([torch.stack([table[-1], table[-2]]), torch.stack([table[-2], table[-1]])]).double()
+    p = torch.softmax(s, 1)
+    want, size = ((p[..., None] * t[None]).sum(1) for t in (v.double(), v.double().abs()))
+    assert ((o.double() - want).abs() <= 2.0 ** -8 * (size + want.abs()) * 1.01 + 2.0 ** -18 * size).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("width", [8, 24, 40, 72, 96, 120])
+@pytest.mark.parametrize("causal", [False, True])
+def test_another_head_stays_out(dev, width, causal):
+    """NaN in the head behind, whose numbers lie where a narrow head's padding would be read: nothing of them arrives, not even times zero"""
+    g = torch.Generator(dev).manual_seed(width)
+    q, k, v, do = (torch.randn(150, 2, width, generator=g, device=dev).bfloat16() for _ in range(4))
+    ends = torch.tensor([0, 33, 150], dtype=torch.int32, device=dev)
+
+    def grads(*t):
+        x = [y.clone().requires_grad_() for y in t[:3]]
+        o = sequence.packed_attention(*x, ends, causal=causal)
+        return [o.detach()] + list(torch.autograd.grad(o, x, t[3]))
+
+    clean = grads(q, k, v, do)
+    for t in (q, k, v, do):
+        t[:, 1] = torch.nan
+    assert all(torch.equal(a[:, 0], b[:, 0]) for a, b in zip(clean, grads(q, k, v, do)))
