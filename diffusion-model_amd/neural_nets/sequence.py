@@ -121,9 +121,10 @@ class LayerNorm(nn.Module):
 
 # ---- attention over packed sequences ----------------------------------------------------------------------------------------
 def _heads(t: Tensor) -> Tensor:
-    """t [tokens, heads, width] as the kernels read it: contiguous heads, 16-byte aligned, no two on each other; copied where it is not"""
+    """t [tokens, heads, width] as the kernels read it: contiguous heads, 16-byte aligned, no two on each other, rows less than 2^24 elements apart;
+    copied where it is not"""
     (rows, heads, width), (row, head, one) = t.shape, t.stride()
-    fits = one == 1 and t.data_ptr() % 16 == 0 and (rows <= 1 or (row >= width and row % 8 == 0)) and (heads <= 1 or (head >= width and head % 8 == 0))
+    fits = one == 1 and t.data_ptr() % 16 == 0 and (rows <= 1 or (width <= row < 1 << 24 and row % 8 == 0)) and (heads <= 1 or (head >= width and head % 8 == 0))
     return t if fits else t.clone(memory_format=torch.contiguous_format)
 
 

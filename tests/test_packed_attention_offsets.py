@@ -43,3 +43,22 @@ def test_another_head_stays_out(dev, width, causal):
     for t in (q, k, v, do):
         t[:, 1] = torch.nan
     assert all(torch.equal(a[:, 0], b[:, 0]) for a, b in zip(clean, grads(q, k, v, do)))
+@pytest.mark.gpu
+@pytest.mark.parametrize("row", [1 << 24, (1 << 24) + 8])
+def test_rows_far_apart_are_copied(dev, row):
+    """rows 2^24 elements apart: past what the kernels read in place"""
+    g = torch.Generator(dev).manual_seed(2)
+    store = torch.zeros(2 * row + 64, device=dev, dtype=torch.bfloat16)
+    far = torch.as_strided(store, (3, 2, 16), (row, 16, 1))
+    near = torch.randn(3, 2, 16, generator=g, device=dev).bfloat16()
+    far.copy_(near)
+    ends = torch.tensor([0, 3], dtype=torch.int32, device=dev)
+    results = []
+    for t in (near, far):
+        x = [t.clone(memory_format=torch.preserve_format) if t is near else t.detach() for _ in range(3)]
+        x = [y.requires_grad_() for y in x]
+        o = sequence.packed_attention(*x, ends, causal=True)
+        results.append([o.detach()] + list(torch.autograd.grad(o, x, near)))
+    assert all(torch.equal(a, b) for a, b in zip(*results))
+
+
