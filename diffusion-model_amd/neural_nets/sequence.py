@@ -48,17 +48,22 @@ _graphs: list = []                   # weak references to the nodes of this modu
 _graphs_lock = threading.RLock()     # (held by sweeps and notes: a node noted between a sweep's look and its end would be lost)
 
 
+def _capturing(t: Tensor) -> bool:
+    with hip.on_device_of(t):
+        return torch.cuda.is_current_stream_capturing()
+
+
 def _note_graph(ctx, *inputs) -> None:
     """All graphs of a leaf share the node that receives its gradient, and that node stays with the stream of the graph that made it.  If that is
     the default stream, autograd makes it wait for a captured backward pass, which no capture survives (nor does the process): so
     the backward pass of a captured graph looks for such a graph, and refuses in time."""
-    ctx.stream, ctx.stale = hip.stream(), False
+    ctx.stream, ctx.stale = hip.stream(inputs[0].get_device()), False        # (of the inputs' device, which need not be the current one)
     if ctx.stream == 0:
         with _graphs_lock:
             _graphs.append(weakref.ref(ctx))
             if len(_graphs) >= 4096:
                 _graphs[:] = [r for r in _graphs if r() is not None]
-    elif torch.cuda.is_current_stream_capturing():
+    elif _capturing(inputs[0]):
         leaves = [t for t in inputs if t is not None and t.requires_grad and t.is_leaf]
         with _graphs_lock:
             noted = list(_graphs)

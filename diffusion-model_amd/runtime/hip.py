@@ -251,9 +251,9 @@ def ptr(t):
     return None if t is None else t.data_ptr()
 
 
-def stream() -> int:
-    """The hipStream_t torch currently enqueues on (so launches are captured by torch.cuda graphs too)."""
-    return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device())      # (torch.cuda.current_stream() wraps it in an object: 2.7 us)
+def stream(device: int = None) -> int:
+    """The hipStream_t torch currently enqueues on (so launches are captured by torch.cuda graphs too), on the current device or the one given."""
+    return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device() if device is None else device)      # (torch.cuda.current_stream() wraps it in an object: 2.7 us)
 
 
 def on_device_of(t):

@@ -31,3 +31,20 @@ def test_a_graph_noted_during_a_sweep_is_kept(monkeypatch):
     assert len(threads) == 1
     threads[0].join(10)
     assert not threads[0].is_alive() and {r() for r in graphs} == {first, late}
+
+
+def test_the_stream_is_that_of_the_inputs_device(monkeypatch):
+    """inputs on the second device, whose current stream is the default one, while the first device is current and on another stream: the graph belongs to
+    the default stream"""
+    class OnSecond:
+        device = torch.device("cuda", 1)
+        requires_grad = is_leaf = True
+        get_device = staticmethod(lambda: 1)
+
+    monkeypatch.setattr(torch._C, "_cuda_getCurrentRawStream", {0: 77, 1: 0}.__getitem__, raising=False)
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: 0)
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: False)
+    monkeypatch.setattr(sequence, "_graphs", [])
+    node = Node()
+    sequence._note_graph(node, OnSecond())
+    assert node.stream == 0 and [r() for r in sequence._graphs] == [node]
