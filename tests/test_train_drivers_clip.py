@@ -27,7 +27,7 @@ def driver(kind, dev, limit):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("kind", sorted(DRIVERS))
-@pytest.mark.parametrize("limit", [1e-3, 1e6])
+@pytest.mark.parametrize("limit", [1e-9, 1e6])             # (gradients of random timesteps differ by orders of magnitude)
 def test_replayed_steps_take_clipped_gradients(dev, kind, limit):
     """weights and first moments after each replay against float64 Adam on gradients times min(1, limit / (norm + 1e-6)), from the state before.
     m' = b1 m + (1 - b1) c g in fp32: 16 roundings (b1, 1 - b1, c and its norm, products, sum).  The weights as in test_grad_clip.py: an update's
