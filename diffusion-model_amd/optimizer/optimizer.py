@@ -137,6 +137,12 @@ class FusedAdam(torch.optim.Optimizer):
                 loss = closure()
         if self._flat is None:
             self._flatten()
+        with hip.on_device_of(self._flat):                # (its streams, whatever device is the current one)
+            self._update(float(grad_scale))
+        bump_weight_epoch()               # the update happened outside torch's view: invalidate cached weight copies
+        return loss
+
+    def _update(self, grad_scale: float) -> None:
         ps = self._params()
         if not torch.cuda.is_current_stream_capturing():
             self.sync_lr()
@@ -145,7 +151,7 @@ class FusedAdam(torch.optim.Optimizer):
         b1, b2 = grp["betas"]
         args = (hip.ptr(self._flat), hip.ptr(g), hip.ptr(self._m), hip.ptr(self._v), hip.ptr(self._ema), self._total,
                 hip.ptr(self._lr), float(grp["lr"]), float(b1), float(b2), float(grp["eps"]), float(grp["weight_decay"]),
-                float(self.ema_decay if self.ema_decay is not None else 0.0), float(grad_scale), hip.ptr(self._step))
+                float(self.ema_decay if self.ema_decay is not None else 0.0), grad_scale, hip.ptr(self._step))
         if self.max_grad_norm is None:
             hip.call("ddpm_adam_step", *args, hip.stream())
         else:
@@ -153,8 +159,6 @@ class FusedAdam(torch.optim.Optimizer):
                 self.grad_norm = torch.zeros((), device=g.device, dtype=torch.float32)
             ops.launch_grad_norm(self._span_off + np.uint64(g.data_ptr()), self._span_n, self._span_kind, hip.NORM_L2, None, self.grad_norm)
             hip.call("ddpm_adam_step_clipped", *args, hip.ptr(self.grad_norm), float(self.max_grad_norm), hip.stream())
-        bump_weight_epoch()               # the update happened outside torch's view: invalidate cached weight copies
-        return loss
 
     @torch.no_grad()
     def step_ranges(self, ranges, last: bool, grad_scale: float = 1.0) -> None:
@@ -166,25 +170,29 @@ class FusedAdam(torch.optim.Optimizer):
             raise RuntimeError("FusedAdam.step_ranges: clipping needs the norm of all gradients, which a step in pieces does not have; use step()")
         if self._flat is None:
             self._flatten()
+        ranges = list(ranges)
+        with hip.on_device_of(self._flat):
+            self._update_ranges(ranges, last, float(grad_scale))
+        if last:
+            if not ranges:
+                raise ValueError("FusedAdam.step_ranges: the last piece of a step cannot be empty")
+            bump_weight_epoch()
+
+    def _update_ranges(self, ranges, last: bool, grad_scale: float) -> None:
         ps = self._params()
         if not torch.cuda.is_current_stream_capturing():
             self.sync_lr()
         g = self._flat_grad(ps)
         grp = self.param_groups[0]
         b1, b2 = grp["betas"]
-        ranges = list(ranges)
         for i, (lo, hi) in enumerate(ranges):
             if not (0 <= lo < hi <= self._total and lo % 4 == 0 and (hi - lo) % 4 == 0):
                 raise ValueError(f"FusedAdam.step_ranges: bad range [{lo}, {hi}) of {self._total}")
             at = lambda t: 0 if t is None else t.data_ptr() + 4 * lo
             hip.call("ddpm_adam_step_range", at(self._flat), at(g), at(self._m), at(self._v), at(self._ema), hi - lo,
                      hip.ptr(self._lr), float(grp["lr"]), float(b1), float(b2), float(grp["eps"]), float(grp["weight_decay"]),
-                     float(self.ema_decay if self.ema_decay is not None else 0.0), float(grad_scale), hip.ptr(self._step),
+                     float(self.ema_decay if self.ema_decay is not None else 0.0), grad_scale, hip.ptr(self._step),
                      int(last and i == len(ranges) - 1), hip.stream())
-        if last:
-            if not ranges:
-                raise ValueError("FusedAdam.step_ranges: the last piece of a step cannot be empty")
-            bump_weight_epoch()
 
 
     # ---- checkpoint interchange ----------------------------------------------------------------------------------------
