@@ -1,6 +1,6 @@
 // Global norm of the gradients of many tensors, and clipping by it (in place, or folded into the optimizer step: param_ops.hip).
 // HBM bound for large models (the norm reads every gradient once, clipping reads and writes it once more); for the denoiser's 27 MB
-// the launches count, so that a call over up to GC_MAX spans of memory is two launches: the table of spans travels in the
+// the launches count, so that a call over up to GC_MAX spans of memory is two launches (beyond that, two for each GC_MAX): the table of spans travels in the
 // kernel arguments (no copy to the device, nothing that a captured graph could find changed), and the second launch adds the
 // first one's partial sums itself, in every workgroup, instead of waiting for a third.
 //   Squares are summed in fp64: the product of two fp32 numbers is exact there, nothing finite overflows, and the cost hides
@@ -191,7 +191,7 @@ template <bool INF> __global__ __launch_bounds__(GC_THREADS) void grad_scale_ker
             constexpr int V = 16 / sizeof(T);
             typedef T vec __attribute__((ext_vector_type(V)));
             // A bf16 tensor is multiplied by the factor rounded to bf16, as torch.nn.utils.clip_grad_norm_ multiplies it: the bits of
-            // that, off by at most 2^-8 in a factor common to the whole tensor.  (An fp16 one is not: fp16 loses factors below 2^-14.)
+            // that, off by at most 2^-8 in a factor common to the whole tensor (and the clipped norm may pass the limit by that).  (An fp16 one is not: fp16 loses factors below 2^-14.)
             const float by = std::is_same<T, bf16>::value ? (float)(bf16)coef : coef;
             gc_chunk(base, n, chunk, [&](vec* p) {
                 vec x = *p;

@@ -119,8 +119,8 @@ __device__ __forceinline__ int pa_scan(int v) {
 }
 
 // The workgroup's rows: `rank` counts the tiles of 128 rows of all sequences, those with the most of the other side's rows first, so that the
-// longest workgroups begin first and short ones fill the end (training batch of 2048 ... 1 causal tokens: forward 104 -> 91 us, backward
-// 370 -> 324).  A lane holds a sequence; the level that the rank falls into is found by bisection: causal, the tile's index within its sequence
+// longest workgroups begin first and short ones fill the end (against the order by slots below, in a row of calls: training batch of 2048 ... 1 causal
+// tokens, forward 108 -> 95 us, backward 360 -> 320; eight of 2048, backward 644 -> 558; but 8192 + 7937 tokens, backward 3.60 -> 3.70 ms).  A lane holds a sequence; the level that the rank falls into is found by bisection: causal, the tile's index within its sequence
 // (queries: a later one sees more keys) or its distance from the end (keys: an earlier one is seen by more queries); otherwise the other
 // side's length in tiles.  More sequences than lanes: by slots, in order.
 template <bool KEYS>
@@ -400,7 +400,7 @@ __global__ __launch_bounds__(256, 2) void pa_fwd_kernel(const PaArgs a) {
         if (t + 1 < tiles) fetch(t + 1);
     };
     // (tiles that the wave has no part in, all behind its own, have a loop of their own: as a branch in this one they made the compiler move the
-    // accumulators to other registers and back for every tile, 64 instructions; 1067 -> 1022 us for 16 K causal tokens)
+    // accumulators to other registers and back for every tile, 64 instructions: 4 % of the time of 16 K causal tokens)
     for (int t = 0; t < mine; ++t) {
         if (BIAS) {
             pa_opaque<DHP>(rp);
@@ -796,8 +796,8 @@ __global__ __launch_bounds__(256) void pa_dtable_kernel(const float* __restrict_
 // backward: dk, dv; a wave owns 32 keys and walks over the queries of every head that shares them
 // ================================================================================================================================
 // Heads of 128: the accumulators and k take 160 registers, so that v is read from LDS and tiles are 32 queries, which leaves room for two
-// workgroups on a CU, each waiting at barriers of its own (one workgroup with v in registers and tiles of 64 queries took 409 us for the batch of
-// 2048 ... 1 causal tokens, 16 heads over 4; this takes 206).
+// workgroups on a CU, each waiting at barriers of its own (one workgroup with v in registers and tiles of 64 queries took twice as long for the batch of
+// 2048 ... 1 causal tokens, 16 heads over 4, which takes 199 to 220 us now).
 // The steps (heads of the group x tiles of queries) may be split over several workgroups, whose 32-bit sums a last launch adds
 // up: few keys with long sequences and shared heads would leave most of the card idle otherwise.
 template <typename T, int DHP, bool BIAS>

@@ -1,6 +1,7 @@
-"""Layers of a conditioning sequence's encoder (the tokens that ConditionalModule attends to): layer norm over the channels of each
-token, and attention over packed sequences of different lengths (causal or not, grouped heads, learned relative position bias), as
-autograd functions and modules on the HIP kernels.  Activations are bf16, fp16 or (layer norm) fp32; parameters are fp32, as
+"""Layers of an encoder of token sequences: layer norm over the channels of each token, and attention over packed sequences of different
+lengths (causal or not, grouped heads, learned relative position bias), as autograd functions and modules on the HIP kernels.  Prompts of one
+length come out of such an encoder as ConditionalModule's key sequence, x.view(prompts, length, width).  ConditionalModule has no mask: prompts of
+different lengths would have to be padded for it, and it would attend to the padding.  Activations are bf16, fp16 or (layer norm) fp32; parameters are fp32, as
 everywhere in this package.  The reference has no such encoder; its ConditionalModule takes the sequence from outside
 (constituent_blocks.py:402-437 there)."""
 from __future__ import annotations
@@ -109,7 +110,7 @@ def layer_norm(x: Tensor, weight: Optional[Tensor] = None, bias: Optional[Tensor
 
 
 class LayerNorm(nn.Module):
-    """nn.LayerNorm over the last axis (same constructor arguments and state_dict keys) on the HIP kernels"""
+    """nn.LayerNorm over the last axis on the HIP kernels: the same state_dict keys; normalized_shape is one number, parameters are fp32"""
 
     def __init__(self, normalized_shape: int, eps: float = 1e-5, elementwise_affine: bool = True, bias: bool = True, device=None):
         super().__init__()
@@ -165,10 +166,12 @@ def packed_attention(q: Tensor, k: Tensor, v: Tensor, ends: Tensor, *, ends_k: O
     ends: int32 [sequences + 1] on the device, ascending from 0: sequence b is the rows ends[b] .. ends[b + 1] - 1 of q (and of k, v, unless
     ends_k gives theirs).  Nothing is read back to the host, and no longest length is needed.  Rows outside of all sequences come out as zeros.
     causal: a query sees the keys up to its own place, counted from the sequences' ends where there are more or fewer keys than queries.
-    A query that sees no key gets zeros.
+    A query that sees no key gets zeros.  A key or value that is not finite may make NaN of every query of its sequence, also of one that does not
+    see it (zero times infinity); other sequences stay as they are.
     bias_table [buckets, heads] (fp32, learned) with bias_buckets [2 far + 1] (int32, relative_position_buckets): adds
     bias_table[bucket of (key's place - query's place), head] to the score.  A bias of -inf hides its distances; finite ones beyond +-5678
-    (2^13 powers of two) count as that.
+    (2^13 powers of two) count as that.  With a bias, a call that will have a gradient of the table keeps more of the probabilities' bits for the
+    product with v than one that will not: the results may differ by a rounding.
     Differentiable once in q, k, v and bias_table (in reverse mode)."""
     for name, t in (("q", q), ("k", k), ("v", v)):
         if t.dim() != 3:

@@ -1,5 +1,5 @@
-"""Global gradient norm and clipping over all parameters of a model in two launches, behind torch's own call signature
-(torch.nn.utils.clip_grad_norm_), which a trainer puts between backward and optimizer.step() (base_trainer.py:226-229 of the
+"""Global gradient norm and clipping over all parameters of a model in a few launches, with the arguments of
+torch.nn.utils.clip_grad_norm_ but `foreach`, which a trainer puts between backward and optimizer.step() (base_trainer.py:226-229 of the
 reference steps without it).  FusedAdam(max_grad_norm=...) folds the same clipping into the optimizer's own pass."""
 from __future__ import annotations
 
@@ -28,7 +28,8 @@ def grad_norm(parameters: Union[Tensor, Iterable[Tensor]], norm_type: float = 2.
 @torch.no_grad()
 def clip_grad_norm_(parameters: Union[Tensor, Iterable[Tensor]], max_norm: float, norm_type: float = 2.0,
                     error_if_nonfinite: bool = False) -> Tensor:
-    """Multiplies all gradients by min(1, max_norm / (norm + 1e-6)) in place and returns the norm they had before.  As in torch, a norm
+    """Multiplies all gradients by min(1, max_norm / (norm + 1e-6)) in place and returns the norm they had before.  bf16 gradients are multiplied
+    by that factor rounded to bf16, as torch does it: their norm may end up to 2^-8 above max_norm.  As in torch, a norm
     that is not finite makes them NaN or zero unless error_if_nonfinite asks for an error: then the norm is read back first (the
     host waits for the GPU) and the gradients stay as they are."""
     grads = _grads(parameters)
