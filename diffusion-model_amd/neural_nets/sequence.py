@@ -46,6 +46,7 @@ def _rows(t: Tensor, c: int) -> Tensor:
 
 
 _graphs: list = []                   # weak references to the nodes of this module's autograd graphs, dead ones swept now and then
+_sweep_at = 4096                     # length of that list at which the next sweep is due
 _graphs_lock = threading.RLock()     # (held by sweeps and notes: a node noted between a sweep's look and its end would be lost)
 
 
@@ -58,12 +59,14 @@ def _note_graph(ctx, *inputs) -> None:
     """All graphs of a leaf share the node that receives its gradient, and that node stays with the stream of the graph that made it.  If that is
     the default stream, autograd makes it wait for a captured backward pass, which no capture survives (nor does the process): so
     the backward pass of a captured graph looks for such a graph, and refuses in time."""
+    global _sweep_at
     ctx.stream, ctx.stale = hip.stream(inputs[0].get_device()), False        # (of the inputs' device, which need not be the current one)
     if ctx.stream == 0:
         with _graphs_lock:
             _graphs.append(weakref.ref(ctx))
-            if len(_graphs) >= 4096:
+            if len(_graphs) >= _sweep_at:
                 _graphs[:] = [r for r in _graphs if r() is not None]
+                _sweep_at = max(4096, 2 * len(_graphs))
     elif _capturing(inputs[0]):
         leaves = [t for t in inputs if t is not None and t.requires_grad and t.is_leaf]
         with _graphs_lock:

@@ -26,6 +26,7 @@ def test_a_graph_noted_during_a_sweep_is_kept(monkeypatch):
 
     graphs = Slow([lambda: None] * 4095)
     monkeypatch.setattr(sequence, "_graphs", graphs)
+    monkeypatch.setattr(sequence, "_sweep_at", 4096)
     first = Node()
     sequence._note_graph(first, torch.zeros(1))
     assert len(threads) == 1
@@ -48,3 +49,25 @@ def test_the_stream_is_that_of_the_inputs_device(monkeypatch):
     node = Node()
     sequence._note_graph(node, OnSecond())
     assert node.stream == 0 and [r() for r in sequence._graphs] == [node]
+
+
+def test_many_living_graphs_are_not_swept_at_every_call(monkeypatch):
+    """with thousands of graphs alive, a sweep frees nothing: the next one waits until the list has doubled"""
+    monkeypatch.setattr(hip, "stream", lambda *a: 0)
+    looks, alive = [0], [Node() for _ in range(12000)]
+
+    class Counted(list):
+        def __setitem__(self, at, value):
+            looks[0] += 1
+            super().__setitem__(at, value)
+
+    monkeypatch.setattr(sequence, "_graphs", Counted())
+    monkeypatch.setattr(sequence, "_sweep_at", 4096)
+    x = torch.zeros(1)
+    for node in alive:
+        sequence._note_graph(node, x)
+    assert [r() for r in sequence._graphs] == alive and looks[0] <= 3
+    del alive[6000:], node
+    for _ in range(30000):                                     # dead ones are swept out all the same
+        sequence._note_graph(Node(), x)
+    assert len(sequence._graphs) < 30000 and [r() for r in sequence._graphs[:6000]] == alive
